@@ -19,10 +19,12 @@ internal static unsafe class Native
         LONNX_E_TIMEOUT = -5, LONNX_E_OOB = -6, LONNX_E_UNSUPPORTED = -7;
     public const int ADD = 0, SUB = 1, MUL = 2, DIV = 3, POW = 4;
     public const int RELU = 0, SQRT = 1, ERF = 2, EXP = 3, GELU_ERF = 4;
+    public const int DT_F32 = 1, DT_F16 = 10, DT_BF16 = 16;
     public const int REDUCE_SUM = 0, REDUCE_MAX = 1, REDUCE_MEAN = 2;
 
     // ---- runtime ----
     [DllImport(Lib)] public static extern int lonnx_ctx_create(int device, out IntPtr ctx);
+    [DllImport(Lib)] public static extern int lonnx_ctx_create_on_stream(int device, IntPtr stream, out IntPtr ctx);
     [DllImport(Lib)] public static extern int lonnx_ctx_destroy(IntPtr ctx);
     [DllImport(Lib)] public static extern int lonnx_ctx_device(IntPtr ctx);
     [DllImport(Lib)] public static extern IntPtr lonnx_ctx_stream(IntPtr ctx);
@@ -58,7 +60,16 @@ internal static unsafe class Native
         int N, int C, int H, int W, int M, int kh, int kw, int sh, int sw, int pt, int pl, int pb, int pr,
         int dh, int dw, int group, int relu);
 
+    [DllImport(Lib)] public static extern int lonnx_quantize_fp8(IntPtr ctx, IntPtr x, int dtype, long rows, long cols,
+        long ldx, int blockRows, IntPtr q, long ldq, IntPtr scale, long lds);
+    [DllImport(Lib)] public static extern int lonnx_gemm_fp8(IntPtr ctx, IntPtr A, long lda, IntPtr scaleA, long ldsA,
+        IntPtr B, long ldb, IntPtr scaleB, long ldsB, IntPtr bias, IntPtr C, int dtypeC, long ldc, int M, int N, int K,
+        int epilogue);
+
     // ---- row kernels ----
+    [DllImport(Lib)] public static extern int lonnx_token_logprobs(IntPtr ctx, IntPtr logits, int dtype, long rows,
+        long vocab, long ld, IntPtr targets, float temperature, IntPtr logprob, IntPtr entropy, int k,
+        IntPtr topLogprob, IntPtr topId);
     [DllImport(Lib)] public static extern int lonnx_softmax_f32(IntPtr ctx, IntPtr x, IntPtr y, long outer, long len, long inner);
     [DllImport(Lib)] public static extern int lonnx_layernorm_f32(IntPtr ctx, IntPtr x, IntPtr res, IntPtr gamma,
         IntPtr beta, float eps, IntPtr y, long rows, int cols);

@@ -47,12 +47,19 @@ enum lonnx_unary_op { LONNX_RELU = 0, LONNX_SQRT = 1, LONNX_ERF = 2, LONNX_EXP =
 enum lonnx_reduce_op { LONNX_REDUCE_SUM = 0, LONNX_REDUCE_MAX = 1, LONNX_REDUCE_MEAN = 2 };
 enum lonnx_epilogue { LONNX_EPI_NONE = 0, LONNX_EPI_RELU = 1, LONNX_EPI_GELU_ERF = 2 };
 
+/* Element types of the entry points that take more than one (ONNX TensorProto codes). */
+enum lonnx_dtype { LONNX_DT_F32 = 1, LONNX_DT_F16 = 10, LONNX_DT_BF16 = 16 };
+
 typedef struct lonnx_ctx lonnx_ctx;
 
 /* ---- runtime -------------------------------------------------------------
  * Replaces the reference's managed storage (DenseTensor<T> over Memory<T>,
  * src/Lokad.Onnx.Tensors/DenseTensor.cs:31-42) with device-resident buffers. */
 LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out);
+/* The same on a stream that the caller owns (a cudaStream_t of `device`; NULL
+ * is the default stream) and keeps until the context is destroyed: work of
+ * the context is then ordered with the caller's own on that stream. */
+LONNX_API int lonnx_ctx_create_on_stream(int device, void *stream, lonnx_ctx **out);
 LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx);
 LONNX_API int lonnx_ctx_device(const lonnx_ctx *ctx);
 LONNX_API void *lonnx_ctx_stream(lonnx_ctx *ctx); /* the cudaStream_t */
@@ -146,11 +153,58 @@ LONNX_API int lonnx_conv2d_f32(lonnx_ctx *ctx, const float *x, const float *w, c
                                int sh, int sw, int pt, int pl, int pb, int pr, int dh, int dw,
                                int group, int relu);
 
+/* Block quantisation to 8-bit float (e4m3, ONNX FLOAT8E4M3FN) of x [rows,
+ * cols] (leading dimension ldx elements; float, float16 or bfloat16), one
+ * fp32 scale per block of block_rows (1: activations, 128: weights) x 128:
+ *   amax = max(2^-96, max |x|), scale = amax / 448, q = e4m3(448 x / amax)
+ * (the nearest e4m3 value, ties to even), so q * scale stands for x.  q: [rows, cols] at
+ * leading dimension ldq bytes (a multiple of 16, from a 16-byte aligned
+ * pointer, where lonnx_gemm_fp8 is to read it); scale: [rows or ceil(rows /
+ * 128), ceil(cols / 128)] at leading dimension lds.  Bytes of q and scale past
+ * a row's end are left as they are.  NaN stays NaN and does not touch its
+ * block's scale; an infinity makes its whole block NaN (scale infinite).  No
+ * counterpart in the reference. */
+LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                 int block_rows, void *q, int64_t ldq, float *scale, int64_t lds);
+/* C = act(A . B^T + bias) with 8-bit float operands (e4m3) and block scales:
+ *   C[m, n] = act(sum_b scaleA[m, b] * scaleB[n / 128, b] *
+ *                 sum_{k in block b} A[m, k] * B[n, k] + bias[n])
+ * over blocks b of 128 along K.  A: [M, K], B: [N, K], K-major; lda and ldb
+ * (bytes) are multiples of 16 and both pointers 16-byte aligned; K is any
+ * number (what lies between K and the leading dimension is not used).  scaleA:
+ * [M, ceil(K / 128)], scaleB: [ceil(N / 128), ceil(K / 128)].  bias: N floats
+ * or NULL.  C: [M, N] of type dtypeC (float, float16, bfloat16) at ldc
+ * elements; what lies past a row's end is left as it is.  Each block's product
+ * is summed by the tensor cores, blocks are scaled and summed in fp32, and the
+ * result is rounded to C's type once, after the epilogue.  Runs without
+ * workspace.  lonnx_gemm_f32's counterpart for quantised weights. */
+LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t lda, const float *scaleA, int64_t ldsA,
+                             const void *B, int64_t ldb, const float *scaleB, int64_t ldsB, const float *bias,
+                             void *C, int dtypeC, int64_t ldc, int M, int N, int K, int epilogue);
+
 /* ---- row kernels -----------------------------------------------------------
  * Softmax over the middle axis of an [outer, len, inner] view: replaces
  * Tensor<float>.Softmax (TensorOps.cs:1312-1330). */
 LONNX_API int lonnx_softmax_f32(lonnx_ctx *ctx, const float *x, float *y, int64_t outer,
                                 int64_t len, int64_t inner);
+/* Scores of tokens from logits [rows, vocab] (leading dimension ld elements;
+ * float, float16 or bfloat16), with z = logits / temperature:
+ *   logprob[r] = z[r, targets[r]] - log sum_v exp(z[r, v])     (NULL: not wanted)
+ *   entropy[r] = -sum_v p[r, v] log p[r, v], p = softmax(z)    (NULL: not wanted)
+ *   top_id / top_logprob [rows, k]: the k likeliest tokens, best first, the
+ *   lowest index first where logits are equal (k = 0: none; at most 32)
+ * one pass, without workspace.  targets (NULL: none) may be given without
+ * logprob; a negative target marks a padding row, which is not read: logprob
+ * 0, entropy 0, top_id -1, top_logprob -inf.  A target past the vocabulary
+ * gives NaN and makes the next lonnx_sync() return LONNX_E_OOB.  Logits of
+ * -inf have no probability; where a row has nothing else, its logprob and
+ * top_logprob are -inf and its entropy 0.  A NaN or +inf logit makes the row's
+ * log-probabilities and entropy NaN; among the alternatives NaN comes last.
+ * temperature: 0.001 to 1000.  The row kernel next to lonnx_softmax_f32 for
+ * vocabularies; no counterpart in the reference. */
+LONNX_API int lonnx_token_logprobs(lonnx_ctx *ctx, const void *logits, int dtype, int64_t rows, int64_t vocab,
+                                   int64_t ld, const int64_t *targets, float temperature, float *logprob,
+                                   float *entropy, int k, float *top_logprob, int64_t *top_id);
 /* Row LayerNorm y = (x+res - mean) / sqrt(var + eps) * gamma + beta over the
  * last axis (cols), res nullable: replaces the ReduceMean -> Sub -> Pow ->
  * ReduceMean -> Add -> Sqrt -> Div -> Mul -> Add node chain

@@ -23,6 +23,7 @@ c_char_p = ctypes.c_char_p
 
 _SIGS = {
     "lonnx_ctx_create": (c_int, [c_int, ctypes.POINTER(c_vp)]),
+    "lonnx_ctx_create_on_stream": (c_int, [c_int, c_vp, ctypes.POINTER(c_vp)]),
     "lonnx_ctx_destroy": (c_int, [c_vp]),
     "lonnx_ctx_device": (c_int, [c_vp]),
     "lonnx_ctx_stream": (c_vp, [c_vp]),
@@ -46,6 +47,11 @@ _SIGS = {
     "lonnx_gemm_f32_noalloc_status": (c_int, [c_vp]),
     "lonnx_matmul_f32": (c_int, [c_vp, c_vp, i64p, c_int, c_vp, i64p, c_int, c_vp]),
     "lonnx_conv2d_f32": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp] + [c_int] * 17),
+    "lonnx_quantize_fp8": (c_int, [c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_i64, c_vp, c_i64]),
+    "lonnx_gemm_fp8": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_int, c_i64,
+                               c_int, c_int, c_int, c_int]),
+    "lonnx_token_logprobs": (c_int, [c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_f32, c_vp, c_vp, c_int, c_vp,
+                                     c_vp]),
     "lonnx_softmax_f32": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64]),
     "lonnx_layernorm_f32": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_f32, c_vp, c_i64, c_int]),
     "lonnx_reduce_f32": (c_int, [c_vp, c_int, c_vp, i64p, c_int, i64p, c_int, c_vp]),

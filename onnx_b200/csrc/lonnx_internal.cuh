@@ -15,7 +15,7 @@
 namespace lonnx {
 
 // Device-side error flags, one int each, read and cleared by lonnx_sync().
-enum DevFlag { FLAG_OOB = 0, FLAG_TIMEOUT = 1, FLAG_COUNT = 4 };
+enum DevFlag { FLAG_OOB = 0, FLAG_TIMEOUT = 1, FLAG_TARGET = 2, FLAG_COUNT = 4 };
 
 struct Allocator {
     // Caching allocator: freed blocks are kept per exact rounded size and
@@ -32,6 +32,7 @@ struct Allocator {
 struct lonnx_ctx {
     int device = 0;
     cudaStream_t stream = nullptr;
+    bool own_stream = true;  // created with the context, destroyed with it
     int *dev_flags = nullptr;  // FLAG_COUNT ints
     int num_sms = 148;
     lonnx::Allocator alloc;

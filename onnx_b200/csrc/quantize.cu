@@ -1,0 +1,285 @@
+// lonnx_quantize_fp8: block quantisation to 8-bit float (e4m3), one fp32
+// scale per block of 128 columns and 1 or 128 rows.
+//
+//   amax  = max(2^-96, max |x| over the block)
+//   scale = amax / 448                      (448: the largest e4m3 value)
+//   q     = e4m3(448 x / amax)              (the quotient's nearest, ties to even)
+//
+// so q * scale stands for x.  2^-96 keeps 448 / amax finite, and a block of
+// zeros quantises to zeros.  The maximum skips NaN, which stays NaN in q; an
+// infinity makes its block's scale infinite and 448 / amax zero, so every
+// element of the block dequantises to NaN.
+//
+// q is the correctly rounded quotient although it comes from an fp32 product
+// p = x * inv, inv = 448 / amax: a point halfway between two e4m3 values has
+// its low 16 mantissa bits zero, so p can be on the wrong side of one only
+// where p's own low bits are zero (about one element in 65536);
+// there the quotient is taken again in double.  It is exact in double
+// at a halfway point, and elsewhere at least 2^-34 away from one, since both
+// sides of 448 X = D A are small integers times powers of two.
+//
+// Bound by HBM: x is read once (into registers, where it waits for its
+// block's maximum), q and the scales are written once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "lonnx_internal.cuh"
+
+namespace {
+
+constexpr int QB = 128;  // columns (and, for weights, rows) of a block
+constexpr float kE4M3Max = 448.0f, kTiny = 0x1p-96f;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// one 16-byte vector of T as floats (4 or 8 of them)
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 &u, float (&f)[16 / sizeof(T)]) {
+    const T *p = reinterpret_cast<const T *>(&u);
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = to_f32(p[i]);
+}
+
+// 448 x / amax as a float that rounds to the same e4m3 value: truncated, with
+// the last bit set where that was not exact (never a halfway point then).
+__device__ __noinline__ float quotient(float x, float amax) {
+    const double t = 448.0 * (double)x / (double)amax;
+    const float f = __double2float_rz(t);
+    return (double)f != t ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+}
+__device__ __forceinline__ bool may_be_halfway(float p) { return (__float_as_uint(p) & 0xffffu) == 0u && p != 0.0f; }
+
+__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, float inv, float amax) {
+    float p[4] = {a * inv, b * inv, c * inv, d * inv};
+    if (may_be_halfway(p[0]) | may_be_halfway(p[1]) | may_be_halfway(p[2]) | may_be_halfway(p[3])) {
+        p[0] = quotient(a, amax);
+        p[1] = quotient(b, amax);
+        p[2] = quotient(c, amax);
+        p[3] = quotient(d, amax);
+    }
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p[0], p[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p[2], p[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+
+// 1 x 128 blocks.  VEC: rows of x start on 16 bytes and rows of q on 16 / sizeof(T)
+// bytes, so a block is 128 * sizeof(T) / 16 lanes of one 16-byte load each
+// (half a warp for 16-bit types); otherwise a warp per block, 4 elements a lane,
+// 32 apart.  Each group of lanes keeps U blocks in flight.
+template <typename T, bool VEC, typename I>
+__global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, I rows, I cols,
+                                                       uint8_t *__restrict__ q, int64_t ldq,
+                                                       float *__restrict__ scale, int64_t lds) {
+    constexpr int VN = VEC ? 16 / (int)sizeof(T) : 4;
+    constexpr int LANES = QB / VN;  // per block
+    constexpr int U = 4;
+    const int lane = threadIdx.x % LANES;
+    const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
+    const I groups = (I)gridDim.x * (blockDim.x / LANES);
+    for (I b0 = (I)blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES; b0 - threadIdx.x / LANES < total;
+         b0 += groups * U) {
+        float v[U][VN];
+        I row[U], kb[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const I b = b0 + u * groups;
+            const bool in = b < total;
+            row[u] = in ? b / nkb : 0;
+            kb[u] = in ? b - row[u] * nkb : nkb;  // nkb: past the row, nothing valid
+            const T *xr = x + (int64_t)row[u] * ldx;
+            const I c = kb[u] * QB;
+            if constexpr (VEC) {
+                const I at = c + lane * VN;
+                if (in && at + VN <= cols) {
+                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xr + at)), v[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) v[u][j] = in && at + j < cols ? to_f32(xr[at + j]) : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VN; ++j) {
+                    const I at = c + lane + 32 * j;
+                    v[u][j] = in && at < cols ? to_f32(xr[at]) : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float m = kTiny;
+#pragma unroll
+            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[u][j]));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (kb[u] >= nkb) continue;
+            const float inv = __fdiv_rn(kE4M3Max, m);
+            if (lane == 0) scale[(int64_t)row[u] * lds + kb[u]] = __fdiv_rn(m, kE4M3Max);
+            uint8_t *qr = q + (int64_t)row[u] * ldq;
+            const I c = kb[u] * QB;
+            if constexpr (VEC) {
+                const I at = c + lane * VN;
+                uint32_t w[VN / 4];
+#pragma unroll
+                for (int j = 0; j < VN / 4; ++j)
+                    w[j] = quant4(v[u][4 * j], v[u][4 * j + 1], v[u][4 * j + 2], v[u][4 * j + 3], inv, m);
+                if (at + VN <= cols) {
+                    if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qr + at) = w[0];
+                    else *reinterpret_cast<uint2 *>(qr + at) = make_uint2(w[0], w[VN / 4 - 1]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                        if (at + j < cols) qr[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+                }
+            } else {
+                const uint32_t w = quant4(v[u][0], v[u][1], v[u][2], v[u][3], inv, m);
+#pragma unroll
+                for (int j = 0; j < VN; ++j) {
+                    const I at = c + lane + 32 * j;
+                    if (at < cols) qr[at] = (uint8_t)(w >> 8 * j);
+                }
+            }
+        }
+    }
+}
+
+// 128 x 128 blocks: a CTA of 8 warps per block, which stays in registers (64
+// values a thread) while the maximum crosses the CTA.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int64_t rows,
+                                                         int64_t cols, uint8_t *__restrict__ q, int64_t ldq,
+                                                         float *__restrict__ scale, int64_t lds) {
+    constexpr int VN = VEC ? 16 / (int)sizeof(T) : 4;
+    constexpr int LANES = QB / VN, TALL = 256 / LANES;  // rows per step
+    constexpr int STEPS = QB / TALL;
+    __shared__ float red[8];
+    const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+    const int64_t nkb = (cols + QB - 1) / QB, total = (rows + QB - 1) / QB * nkb;
+    for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
+        const int64_t rb = b / nkb, kb = b - rb * nkb;
+        const T *xb = x + rb * QB * ldx + kb * QB;
+        uint8_t *qb = q + rb * QB * ldq + kb * QB;
+        const int nr = (int)min((int64_t)QB, rows - rb * QB), nc = (int)min((int64_t)QB, cols - kb * QB);
+        float v[STEPS][VN];
+        float m = kTiny;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int r = r0 + s * TALL;
+            const T *xr = xb + (int64_t)r * ldx;
+            if constexpr (VEC) {
+                const int at = lane * VN;
+                if (r < nr && at + VN <= nc) {
+                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xr + at)), v[s]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) v[s][j] = r < nr && at + j < nc ? to_f32(xr[at + j]) : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VN; ++j)
+                    v[s][j] = r < nr && lane + 32 * j < nc ? to_f32(xr[lane + 32 * j]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[s][j]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+        __syncthreads();
+        const float inv = __fdiv_rn(kE4M3Max, m);
+        if (threadIdx.x == 0) scale[rb * lds + kb] = __fdiv_rn(m, kE4M3Max);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int r = r0 + s * TALL;
+            if (r >= nr) continue;
+            uint8_t *qr = qb + (int64_t)r * ldq;
+            uint32_t w[VN / 4];
+#pragma unroll
+            for (int j = 0; j < VN / 4; ++j)
+                w[j] = quant4(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], inv, m);
+            if constexpr (VEC) {
+                const int at = lane * VN;
+                if (at + VN <= nc) {
+                    if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qr + at) = w[0];
+                    else *reinterpret_cast<uint2 *>(qr + at) = make_uint2(w[0], w[VN / 4 - 1]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                        if (at + j < nc) qr[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VN; ++j)
+                    if (lane + 32 * j < nc) qr[lane + 32 * j] = (uint8_t)(w[0] >> 8 * j);
+            }
+        }
+    }
+}
+
+template <typename T>
+int quantize(lonnx_ctx *ctx, const void *xv, int64_t rows, int64_t cols, int64_t ldx, int block_rows, uint8_t *q,
+             int64_t ldq, float *scale, int64_t lds) {
+    const T *x = static_cast<const T *>(xv);
+    constexpr int VN = 16 / (int)sizeof(T);
+    const bool vec = ((uintptr_t)x & 15) == 0 && ldx % VN == 0 && ((uintptr_t)q & (VN - 1)) == 0 && ldq % VN == 0;
+    const int64_t nkb = (cols + QB - 1) / QB;
+    cudaStream_t st = ctx->stream;
+    if (block_rows == 1) {
+        const int64_t total = rows * nkb, per_cta = 256 / (vec ? QB / VN : 32);
+        const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, (int64_t)ctx->num_sms * 32);
+        // 32-bit indices (one 32-bit division per block) where blocks and columns allow it
+        const bool small = total + (int64_t)grid * per_cta * 4 < (1ll << 31) && cols < (1ll << 30);
+        if (vec && small)
+            k_quantize_rows<T, true, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
+        else if (vec)
+            k_quantize_rows<T, true, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        else if (small)
+            k_quantize_rows<T, false, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
+        else
+            k_quantize_rows<T, false, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+    } else {
+        const int64_t total = (rows + QB - 1) / QB * nkb;
+        const unsigned grid = (unsigned)std::min<int64_t>(total, 1ll << 30);
+        if (vec)
+            k_quantize_blocks<T, true><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        else
+            k_quantize_blocks<T, false><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+    }
+    LONNX_CHECK_LAUNCH(ctx);
+    return LONNX_OK;
+}
+
+}  // namespace
+
+using namespace lonnx;
+
+extern "C" LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols,
+                                            int64_t ldx, int block_rows, void *q, int64_t ldq, float *scale,
+                                            int64_t lds) {
+    const int es = dtype == LONNX_DT_F32 ? 4 : dtype == LONNX_DT_F16 || dtype == LONNX_DT_BF16 ? 2 : 0;
+    if (!es) return set_error(LONNX_E_UNSUPPORTED, "quantize_fp8: input type %d (float, float16 and bfloat16 are supported)", dtype);
+    if (block_rows != 1 && block_rows != QB)
+        return set_error(LONNX_E_BADARG, "quantize_fp8: blocks of %d rows (1 or 128 are supported)", block_rows);
+    if (rows < 0 || cols < 0) return set_error(LONNX_E_BADARG, "quantize_fp8: negative size");
+    if (ldx < cols || ldq < cols || lds < (cols + QB - 1) / QB)
+        return set_error(LONNX_E_SHAPE, "quantize_fp8: a leading dimension is smaller than its row");
+    if (((uintptr_t)x & (es - 1)) || ((uintptr_t)scale & 3))
+        return set_error(LONNX_E_BADARG, "quantize_fp8: a pointer is not aligned to its element type");
+    int rc = device_guard(ctx);
+    if (rc) return rc;
+    if (rows == 0 || cols == 0) return LONNX_OK;
+    if (!x || !q || !scale) return set_error(LONNX_E_BADARG, "quantize_fp8: null pointer");
+    uint8_t *qb = static_cast<uint8_t *>(q);
+    if (dtype == LONNX_DT_F32) return quantize<float>(ctx, x, rows, cols, ldx, block_rows, qb, ldq, scale, lds);
+    if (dtype == LONNX_DT_F16) return quantize<__half>(ctx, x, rows, cols, ldx, block_rows, qb, ldq, scale, lds);
+    return quantize<__nv_bfloat16>(ctx, x, rows, cols, ldx, block_rows, qb, ldq, scale, lds);
+}

@@ -143,7 +143,7 @@ extern "C" {
 
 LONNX_API const char *lonnx_last_error(void) { return g_last_error.c_str(); }
 
-LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out) {
+static int ctx_create(int device, bool own_stream, cudaStream_t stream, lonnx_ctx **out) {
     if (!out) return set_error(LONNX_E_BADARG, "null output pointer");
     int n = 0;
     cudaError_t e = cudaGetDeviceCount(&n);
@@ -162,20 +162,38 @@ LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out) {
     c->device = device;
     c->num_sms = prop.multiProcessorCount;
     if (const char *lim = getenv("LONNX_MEM_LIMIT")) c->alloc.limit = strtoull(lim, nullptr, 10);
-    e = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
-    if (e != cudaSuccess) {
-        delete c;
-        return cuda_error(e, "cudaStreamCreate");
+    c->stream = stream;
+    c->own_stream = own_stream;
+    if (own_stream) {
+        e = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
+        if (e != cudaSuccess) {
+            delete c;
+            return cuda_error(e, "cudaStreamCreate");
+        }
     }
     e = cudaMalloc(&c->dev_flags, sizeof(int) * FLAG_COUNT);
     if (e == cudaSuccess) e = cudaMemset(c->dev_flags, 0, sizeof(int) * FLAG_COUNT);
     if (e != cudaSuccess) {
-        cudaStreamDestroy(c->stream);
+        if (own_stream) cudaStreamDestroy(c->stream);
         delete c;
         return cuda_error(e, "cudaMalloc(flags)");
     }
     *out = c;
     return LONNX_OK;
+}
+
+LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out) { return ctx_create(device, true, nullptr, out); }
+
+LONNX_API int lonnx_ctx_create_on_stream(int device, void *stream, lonnx_ctx **out) {
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // the default streams belong to every device; any other to the one it was made on
+    if (s != nullptr && s != cudaStreamLegacy && s != cudaStreamPerThread) {
+        int of = -1;
+        const cudaError_t e = cudaStreamGetDevice(s, &of);
+        if (e != cudaSuccess) return cuda_error(e, "cudaStreamGetDevice");
+        if (of != device) return set_error(LONNX_E_BADARG, "stream of device %d given for device %d", of, device);
+    }
+    return ctx_create(device, false, s, out);
 }
 
 LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx) {
@@ -185,7 +203,7 @@ LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx) {
     for (auto &kv : ctx->alloc.free_blocks) cudaFree(kv.second);
     for (auto &kv : ctx->alloc.live) cudaFree(kv.first);
     cudaFree(ctx->dev_flags);
-    cudaStreamDestroy(ctx->stream);
+    if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return LONNX_OK;
 }
@@ -249,11 +267,12 @@ LONNX_API int lonnx_sync(lonnx_ctx *ctx) {
     LONNX_CUDA(cudaStreamSynchronize(ctx->stream));
     int flags[FLAG_COUNT];
     LONNX_CUDA(cudaMemcpy(flags, ctx->dev_flags, sizeof(flags), cudaMemcpyDeviceToHost));
-    if (flags[FLAG_OOB] || flags[FLAG_TIMEOUT]) {
+    if (flags[FLAG_OOB] || flags[FLAG_TIMEOUT] || flags[FLAG_TARGET]) {
         LONNX_CUDA(cudaMemset(ctx->dev_flags, 0, sizeof(flags)));
         if (flags[FLAG_TIMEOUT])
             return set_error(LONNX_E_TIMEOUT, "a device-side pipeline wait expired (code %d)", flags[FLAG_TIMEOUT]);
-        return set_error(LONNX_E_OOB, "Gather: an index was outside the bounds of the data axis");
+        if (flags[FLAG_OOB]) return set_error(LONNX_E_OOB, "Gather: an index was outside the bounds of the data axis");
+        return set_error(LONNX_E_OOB, "token_logprobs: a target was outside the vocabulary");
     }
     return LONNX_OK;
 }

@@ -14,7 +14,13 @@ import numpy as np
 
 from . import _native as N
 
-ONNX_DTYPE = {np.dtype(np.float32): 1, np.dtype(np.int64): 7, np.dtype(np.int32): 6,
+# Element types numpy has no name for: one field holding the bits (a host copy
+# is read as `a.view(np.uint16)` or `a.view(np.uint8)`).
+BFLOAT16 = np.dtype([("bfloat16", "<u2")])
+FLOAT8E4M3 = np.dtype([("float8e4m3fn", "u1")])
+
+ONNX_DTYPE = {np.dtype(np.float16): 10, BFLOAT16: 16, FLOAT8E4M3: 17,
+              np.dtype(np.float32): 1, np.dtype(np.int64): 7, np.dtype(np.int32): 6,
               np.dtype(np.uint8): 2, np.dtype(np.bool_): 9, np.dtype(np.float64): 11}
 NP_DTYPE = {v: k for k, v in ONNX_DTYPE.items()}
 
@@ -25,9 +31,14 @@ class Context:
     _default = {}
     _lock = threading.Lock()
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
+        """``stream``: a CUDA stream of the caller's (its handle, 0 the default
+        stream) to run on and to be ordered with; None makes one."""
         h = ctypes.c_void_p()
-        N.check(N.lib.lonnx_ctx_create(device, ctypes.byref(h)))
+        if stream is None:
+            N.check(N.lib.lonnx_ctx_create(device, ctypes.byref(h)))
+        else:
+            N.check(N.lib.lonnx_ctx_create_on_stream(device, stream, ctypes.byref(h)))
         self.handle = h
         self.device = device
 
