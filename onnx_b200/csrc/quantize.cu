@@ -12,11 +12,11 @@
 //
 // q is the correctly rounded quotient although it comes from an fp32 product
 // p = x * inv, inv = 448 / amax: a point halfway between two e4m3 values has
-// its low 16 mantissa bits zero, so p can be on the wrong side of one only
-// where p's own low bits are zero (about one element in 65536);
-// there the quotient is taken again in double.  It is exact in double
-// at a halfway point, and elsewhere at least 2^-34 away from one, since both
-// sides of 448 X = D A are small integers times powers of two.
+// its low 16 bits zero, and p is within two steps of the quotient (half a step
+// from each of its two roundings, at most twice that across a power of two),
+// so p can be on the wrong side only where its low bits are within 2 of zero
+// (one element in 13000).  There the quotient is taken as p + e, with the
+// remainders of both roundings in e.
 //
 // Bound by HBM: x is read once (into registers, where it waits for its
 // block's maximum), q and the scales are written once.
@@ -45,102 +45,116 @@ __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[16 / sizeof(T)
     for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = to_f32(p[i]);
 }
 
-// 448 x / amax as a float that rounds to the same e4m3 value: truncated, with
-// the last bit set where that was not exact (never a halfway point then).
-__device__ __noinline__ float quotient(float x, float amax) {
-    const double t = 448.0 * (double)x / (double)amax;
-    const float f = __double2float_rz(t);
-    return (double)f != t ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+// One block's factors: inv = 448 / amax, and what that rounding left, relative.
+struct Factor {
+    float inv, rest;
+};
+__device__ __forceinline__ Factor factor(float amax) {
+    const float inv = __fdiv_rn(kE4M3Max, amax);
+    return {inv, __fmaf_rn(-amax, inv, kE4M3Max) * (1.0f / kE4M3Max)};
 }
-__device__ __forceinline__ bool may_be_halfway(float p) { return (__float_as_uint(p) & 0xffffu) == 0u && p != 0.0f; }
 
-__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, float inv, float amax) {
-    float p[4] = {a * inv, b * inv, c * inv, d * inv};
+__device__ __forceinline__ bool may_be_halfway(float p) { return ((__float_as_uint(p) + 2u) & 0xffffu) <= 4u; }
+
+// A float that rounds to the same e4m3 value as 448 x / amax = p + e: the sum,
+// with its last bit set where it is not exact, which no halfway point has.  e
+// is right to 2^-46 of p; a quotient is a halfway point or, as 448 X = D A has
+// integers under 2^33 times powers of two on both sides, 2^-34 away from it.
+__device__ __forceinline__ float quotient(float x, float p, Factor f) {
+    const float e = __fmaf_rn(x, f.inv, -p) + p * f.rest;
+    const float s = p + e, left = (p - s) + e;
+    const uint32_t b = __float_as_uint(s);
+    const bool inexact = fabsf(left) > 0x1p-40f * fabsf(s) && !(b & 1);
+    return !inexact ? s : __uint_as_float((left > 0.0f) == (s > 0.0f) ? b + 1 : b - 1);
+}
+
+__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, Factor f) {
+    float p[4] = {a * f.inv, b * f.inv, c * f.inv, d * f.inv};
     if (may_be_halfway(p[0]) | may_be_halfway(p[1]) | may_be_halfway(p[2]) | may_be_halfway(p[3])) {
-        p[0] = quotient(a, amax);
-        p[1] = quotient(b, amax);
-        p[2] = quotient(c, amax);
-        p[3] = quotient(d, amax);
+        // (most often zeros, which stay)
+        if (p[0] != 0.0f && may_be_halfway(p[0])) p[0] = quotient(a, p[0], f);
+        if (p[1] != 0.0f && may_be_halfway(p[1])) p[1] = quotient(b, p[1], f);
+        if (p[2] != 0.0f && may_be_halfway(p[2])) p[2] = quotient(c, p[2], f);
+        if (p[3] != 0.0f && may_be_halfway(p[3])) p[3] = quotient(d, p[3], f);
     }
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p[0], p[1]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p[2], p[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
 
-// 1 x 128 blocks.  VEC: rows of x start on 16 bytes and rows of q on 16 / sizeof(T)
-// bytes, so a block is 128 * sizeof(T) / 16 lanes of one 16-byte load each
-// (half a warp for 16-bit types); otherwise a warp per block, 4 elements a lane,
-// 32 apart.  Each group of lanes keeps U blocks in flight.
+// 1 x 128 blocks, 8 lanes to a block and 16 elements to a lane, so that the
+// block's two divisions and the shuffles for its maximum are shared by 16
+// elements (a warp to a block of floats, 4 elements a lane, took 72 us instead
+// of 48 at 32768 x 1536: it was bound by instructions).  VEC: rows of x start
+// on 16 bytes and rows of q on 16 / sizeof(T) bytes, and a lane's elements are
+// 16-byte vectors, 8 vectors apart; otherwise single elements, 8 apart.
 template <typename T, bool VEC, typename I>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, I rows, I cols,
                                                        uint8_t *__restrict__ q, int64_t ldq,
                                                        float *__restrict__ scale, int64_t lds) {
-    constexpr int VN = VEC ? 16 / (int)sizeof(T) : 4;
-    constexpr int LANES = QB / VN;  // per block
-    constexpr int U = 4;
+    constexpr int VN = VEC ? 16 / (int)sizeof(T) : 1;  // elements of one access
+    constexpr int LANES = 8, NV = QB / LANES / VN;
     const int lane = threadIdx.x % LANES;
     const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
-    const I groups = (I)gridDim.x * (blockDim.x / LANES);
-    for (I b0 = (I)blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES; b0 - threadIdx.x / LANES < total;
-         b0 += groups * U) {
-        float v[U][VN];
-        I row[U], kb[U];
+    const I first = (I)blockIdx.x * (256 / LANES), step = (I)gridDim.x * (256 / LANES);
+    for (I base = first; base < total; base += step) {
+        const I b = base + (I)(threadIdx.x / LANES);
+        const bool in = b < total;
+        const I row = in ? b / nkb : 0, kb = in ? b - row * nkb : 0;
+        const I c = kb * QB;
+        const int nc = !in ? 0 : cols - c < QB ? (int)(cols - c) : QB;
+        const T *xb = x + (int64_t)row * ldx + c;
+        float v[NV][VN];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const I b = b0 + u * groups;
-            const bool in = b < total;
-            row[u] = in ? b / nkb : 0;
-            kb[u] = in ? b - row[u] * nkb : nkb;  // nkb: past the row, nothing valid
-            const T *xr = x + (int64_t)row[u] * ldx;
-            const I c = kb[u] * QB;
+        for (int i = 0; i < NV; ++i) {
+            const int at = (lane + LANES * i) * VN;
             if constexpr (VEC) {
-                const I at = c + lane * VN;
-                if (in && at + VN <= cols) {
-                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xr + at)), v[u]);
+                if (at + VN <= nc) {
+                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xb + at)), v[i]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < VN; ++j) v[u][j] = in && at + j < cols ? to_f32(xr[at + j]) : 0.0f;
+                    for (int j = 0; j < VN; ++j) v[i][j] = at + j < nc ? to_f32(xb[at + j]) : 0.0f;
                 }
             } else {
-#pragma unroll
-                for (int j = 0; j < VN; ++j) {
-                    const I at = c + lane + 32 * j;
-                    v[u][j] = in && at < cols ? to_f32(xr[at]) : 0.0f;
-                }
+                v[i][0] = at < nc ? to_f32(xb[at]) : 0.0f;
             }
         }
+        float m = kTiny;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float m = kTiny;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[u][j]));
+            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[i][j]));
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (kb[u] >= nkb) continue;
-            const float inv = __fdiv_rn(kE4M3Max, m);
-            if (lane == 0) scale[(int64_t)row[u] * lds + kb[u]] = __fdiv_rn(m, kE4M3Max);
-            uint8_t *qr = q + (int64_t)row[u] * ldq;
-            const I c = kb[u] * QB;
-            if constexpr (VEC) {
-                const I at = c + lane * VN;
+        for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!in) continue;
+        const Factor f = factor(m);
+        if (lane == 0) scale[(int64_t)row * lds + kb] = __fdiv_rn(m, kE4M3Max);
+        uint8_t *qb = q + (int64_t)row * ldq + c;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int at = (lane + LANES * i) * VN;
                 uint32_t w[VN / 4];
 #pragma unroll
                 for (int j = 0; j < VN / 4; ++j)
-                    w[j] = quant4(v[u][4 * j], v[u][4 * j + 1], v[u][4 * j + 2], v[u][4 * j + 3], inv, m);
-                if (at + VN <= cols) {
-                    if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qr + at) = w[0];
-                    else *reinterpret_cast<uint2 *>(qr + at) = make_uint2(w[0], w[VN / 4 - 1]);
+                    w[j] = quant4(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3], f);
+                if (at + VN <= nc) {
+                    if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qb + at) = w[0];
+                    else *reinterpret_cast<uint2 *>(qb + at) = make_uint2(w[0], w[VN / 4 - 1]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < VN; ++j)
-                        if (at + j < cols) qr[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+                        if (at + j < nc) qb[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
                 }
-            } else {
-                const uint32_t w = quant4(v[u][0], v[u][1], v[u][2], v[u][3], inv, m);
+            }
+        } else {
 #pragma unroll
-                for (int j = 0; j < VN; ++j) {
-                    const I at = c + lane + 32 * j;
-                    if (at < cols) qr[at] = (uint8_t)(w >> 8 * j);
+            for (int i = 0; i < NV; i += 4) {
+                const uint32_t w = quant4(v[i][0], v[i + 1][0], v[i + 2][0], v[i + 3][0], f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = lane + LANES * (i + j);
+                    if (at < nc) qb[at] = (uint8_t)(w >> 8 * j);
                 }
             }
         }
@@ -195,7 +209,7 @@ __global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x
 #pragma unroll
         for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
         __syncthreads();
-        const float inv = __fdiv_rn(kE4M3Max, m);
+        const Factor f = factor(m);
         if (threadIdx.x == 0) scale[rb * lds + kb] = __fdiv_rn(m, kE4M3Max);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -205,7 +219,7 @@ __global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x
             uint32_t w[VN / 4];
 #pragma unroll
             for (int j = 0; j < VN / 4; ++j)
-                w[j] = quant4(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], inv, m);
+                w[j] = quant4(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], f);
             if constexpr (VEC) {
                 const int at = lane * VN;
                 if (at + VN <= nc) {
@@ -234,10 +248,10 @@ int quantize(lonnx_ctx *ctx, const void *xv, int64_t rows, int64_t cols, int64_t
     const int64_t nkb = (cols + QB - 1) / QB;
     cudaStream_t st = ctx->stream;
     if (block_rows == 1) {
-        const int64_t total = rows * nkb, per_cta = 256 / (vec ? QB / VN : 32);
+        const int64_t total = rows * nkb, per_cta = 256 / 8;
         const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, (int64_t)ctx->num_sms * 32);
         // 32-bit indices (one 32-bit division per block) where blocks and columns allow it
-        const bool small = total + (int64_t)grid * per_cta * 4 < (1ll << 31) && cols < (1ll << 30);
+        const bool small = total + (int64_t)grid * per_cta < (1ll << 31) && cols < (1ll << 30);
         if (vec && small)
             k_quantize_rows<T, true, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
         else if (vec)
