@@ -2,17 +2,37 @@
 // and one fp32 scale per 1 x 128 block of A and per 128 x 128 block of B:
 //
 //   C[m, n] = act(sum_b sA[m, b] * sB[n / 128, b] * sum_{k in block b} A[m, k] B[n, k] + bias[n])
+//
+// The tensor cores (tcgen05.mma kind::f8f6f4) sum one block of 128 columns of
+// K into TMEM; warps read that sum back, scale it and add it to fp32 registers
+// while the next block runs into the other of two TMEM buffers.  So a block's
+// products are exact fp32-accumulated sums of 128 terms, and scales of any
+// value (not only powers of two) cost one FMA an element and block.
+//
+// Two kernels.  k_fp8_wide: tiles of 128 rows of A x BN rows of B, for
+// problems that fill the GPU with them.  k_fp8_split: B's rows as the tensor
+// core's 128 and 16 to 128 rows of A as its columns, K split over the CTAs of
+// a cluster that add their sums over distributed shared memory: for few rows,
+// where the weights' bytes and the latency count.  Neither needs a workspace.
+#include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include <algorithm>
 
 #include "lonnx_internal.cuh"
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int KB = 128;
+using namespace lonnx::tc;
+
+constexpr int KB = 128;  // columns of a block: one 128-byte row of the swizzled tiles
+constexpr int BM = 128;  // rows of a tile on the tensor core
+constexpr int kTile = BM * KB;  // bytes of 128 rows of one block
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
@@ -23,52 +43,598 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ float from_e4m3(uint8_t b) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+__device__ __forceinline__ float activate(float v, int epi) {
+    if (epi == LONNX_EPI_RELU) return v > 0.0f ? v : 0.0f;  // NaN gives 0, as lonnx_gemm_f32's
+    return epi == LONNX_EPI_GELU_ERF ? lonnx_gelu_fast(v) : v;
 }
 
-// A 16 x 16 tile of C per CTA, one element per thread, one 128-block at a time
-template <typename T>
-__global__ void __launch_bounds__(256) k_gemm_fp8_plain(const uint8_t *__restrict__ A, int64_t lda,
-                                                        const float *__restrict__ sA, int64_t ldsA,
-                                                        const uint8_t *__restrict__ B, int64_t ldb,
-                                                        const float *__restrict__ sB, int64_t ldsB,
-                                                        const float *__restrict__ bias, T *__restrict__ C, int64_t ldc,
-                                                        int M, int N, int K, int epi) {
-    __shared__ float ta[16][KB + 1], tb[16][KB + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int m = blockIdx.y * 16 + ty, n = blockIdx.x * 16 + tx;
-    float acc = 0.0f;
-    for (int b = 0; b * KB < K; ++b) {
-        for (int i = threadIdx.x; i < 16 * KB; i += 256) {
-            const int r = i / KB, c = b * KB + i % KB;
-            const int64_t ra = blockIdx.y * 16 + r, rb = blockIdx.x * 16 + r;
-            ta[r][i % KB] = ra < M && c < K ? from_e4m3(A[ra * lda + c]) : 0.0f;
-            tb[r][i % KB] = rb < N && c < K ? from_e4m3(B[rb * ldb + c]) : 0.0f;
+// D[tmem] (+)= A[smem desc] x B[smem desc], kind::f8f6f4 (32 columns of K), one CTA
+__device__ __forceinline__ void mma_fp8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor for kind::f8f6f4: D fp32 [4,6)=1, A and B e4m3
+// ([7,10) and [10,13) = 0), both K-major, N >> 3 at [17,23), M >> 4 at [24,29).
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// two fp32 FMAs in one instruction: c += a * s
+__device__ __forceinline__ void fma2(uint64_t &c, uint64_t a, uint64_t s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(s));
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t pack2u(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+// Four blocks' scales of one row, from block b (0 past the row's end)
+__device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int b, int nkb, bool valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = valid && b + i < nkb ? __ldg(row + b + i) : 0.0f;
+}
+
+// ---- wide tiles -----------------------------------------------------------------
+//
+// CTA = 10 warps, one per SM, walking tiles of 128 x BN:
+//   warps 0-7  drain: each thread one row x BN / 2 columns in registers; then
+//              the epilogue, 128 bytes of a row at a time through 4 KB of
+//              shared memory per warp and out by TMA (or, where rows of C do
+//              not start on 16 bytes, by coalesced element stores)
+//   warp 8     TMA producer, warp 9 MMA issuer (and TMEM)
+template <int BN>
+struct Wide {
+    static constexpr int STAGE = kTile + BN * KB;
+    static constexpr int S = BN == 256 ? 4 : 6;
+    static constexpr int STAGING = 8 * 4096;
+    static constexpr int SMEM = 1024 + S * STAGE + STAGING + (2 * S + 5) * 8 + 8;
+    static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
+};
+constexpr int kWideThreads = 320;
+constexpr int W_TMA = 8, W_MMA = 9;
+
+// Tiles in groups of 16 rows of tiles, column by column within a group, so
+// that the CTAs at work share both operands' tiles in L2.
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int &tm, int &tn) {
+    constexpr int GROUP = 16;
+    const int per = GROUP * tiles_n, g = t / per, first = g * GROUP;
+    const int h = min(GROUP, tiles_m - first), r = t - g * per;
+    tn = r / h;
+    tm = first + r - tn * h;
+}
+
+template <int BN, typename T>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    k_fp8_wide(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+               const __grid_constant__ CUtensorMap mapC, const float *__restrict__ sA, int64_t ldsA,
+               const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
+               int64_t ldc, int M, int N, int nkb, int epi, int by_tma, int *flags) {
+    using W = Wide<BN>;
+    constexpr int S = W::S, COLS = BN / 2;
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *staging = base + S * W::STAGE;
+    uint64_t *bar0 = reinterpret_cast<uint64_t *>(staging + W::STAGING);
+    const uint32_t bars = smem_u32(bar0);
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (S + s); };
+    auto tfull = [&](int b) { return bars + 8 * (2 * S + b); };
+    auto tempty = [&](int b) { return bars + 8 * (2 * S + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * S + 4);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + 2 * S + 5);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + 2 * S + 5) + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
         }
-        __syncthreads();
-        float part = 0.0f;
-        for (int k = 0; k < KB; ++k) part = fmaf(ta[ty][k], tb[tx][k], part);
-        if (m < M && n < N) acc = fmaf(part, sA[m * ldsA + b] * sB[(int64_t)(n / KB) * ldsB + b], acc);
-        __syncthreads();
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull(b), 1);
+            mbar_init(tempty(b), 8);
+        }
+        mbar_init(drained, 1);
+        fence_mbar_init();
     }
-    if (m < M && n < N) {
-        if (bias) acc += bias[n];
-        if (epi == LONNX_EPI_RELU) acc = acc > 0.0f ? acc : 0.0f;
-        else if (epi == LONNX_EPI_GELU_ERF) acc = lonnx_gelu_fast(acc);
-        C[m * ldc + n] = from_f32<T>(acc);
+    if (warp == W_MMA) {
+        tmem_alloc(smem_u32(tmem_slot), 2 * BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+    bool ok = true;
+    int issued = 0;  // TMA: stages filled
+    if (warp == W_TMA) {
+        if (lane == 0) {
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                int tm, tn;
+                tile_at(t, tiles_m, tiles_n, tm, tn);
+                for (int b = 0; b < nkb; ++b, ++issued) {
+                    const int s = issued % S;
+                    if (!mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    const uint32_t at = smem_u32(base + s * W::STAGE);
+                    mbar_arrive_expect_tx(full(s), W::STAGE);
+                    tma_load_2d(at, &mapA, full(s), b * KB, tm * BM);
+                    tma_load_2d(at + kTile, &mapB, full(s), b * KB, tn * BN);
+                }
+            }
+        }
+    } else if (warp == W_MMA) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(BM, BN);
+            int j = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                for (int b = 0; b < nkb; ++b, ++j) {
+                    const int s = j % S, buf = j & 1;
+                    if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait(full(s), (j / S) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t da = smem_desc_sw128(smem_u32(base + s * W::STAGE));
+                    const uint64_t db = smem_desc_sw128(smem_u32(base + s * W::STAGE + kTile));
+#pragma unroll
+                    for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, k > 0);
+                    mma_commit(empty(s));
+                    mma_commit(tfull(buf));
+                }
+            }
+        }
+    } else {
+        const int q = warp & 3, half = warp >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
+        uint8_t *stage = staging + warp * 4096;
+        int j = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            int tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            const int row = tm * BM + q * 32 + lane, col0 = tn * BN + half * COLS;
+            const bool valid = row < M;
+            const float *ra = sA + (int64_t)(valid ? row : 0) * ldsA;
+            // (a half past N has no scale row: its columns are not written)
+            const float *rb = sB + (int64_t)(col0 < N ? col0 / KB : 0) * ldsB;
+            uint64_t acc[COLS / 2];
+#pragma unroll
+            for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
+            float sa[4], sb[4], na[4], nb[4];
+            load_scales(na, ra, 0, nkb, valid);
+            load_scales(nb, rb, 0, nkb, true);
+            for (int b0 = 0; b0 < nkb && ok; b0 += 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sa[i] = na[i], sb[i] = nb[i];
+                load_scales(na, ra, b0 + 4, nkb, valid);
+                load_scales(nb, rb, b0 + 4, nkb, true);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (b0 + i >= nkb) break;
+                    const int buf = j & 1;
+                    // (one answer for the warp: its next steps are collective)
+                    if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
+                    ++j;
+                    tc_fence_after();
+                    const float s = sa[i] * sb[i];
+                    const uint64_t s2 = pack2(s, s);
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld_32x32b_x32(lanes + buf * BN + c * 32, r);
+                        tmem_ld_wait();
+                        if (c == COLS / 32 - 1) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(tempty(buf));
+                        }
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) fma2(acc[c * 16 + u], pack2u(r[2 * u], r[2 * u + 1]), s2);
+                    }
+                }
+            }
+            if (!ok) break;
+            // 128 bytes of each of the warp's 32 rows at a time
+            constexpr int PIECE = 128 / (int)sizeof(T);
+#pragma unroll
+            for (int p = 0; p < COLS / PIECE; ++p) {
+                if (lane == 0) bulk_wait_group_read0();
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {  // 16-byte chunks of this lane's row
+                    constexpr int CN = 16 / (int)sizeof(T);
+                    T out[CN];
+#pragma unroll
+                    for (int u = 0; u < CN; u += 2) {
+                        const int e = p * PIECE + c * CN + u;
+                        float2 v = unpack2(acc[e / 2]);
+                        if (bias) {
+                            v.x += __ldg(bias + min(col0 + e, N - 1));
+                            v.y += __ldg(bias + min(col0 + e + 1, N - 1));
+                        }
+                        out[u] = from_f32<T>(activate(v.x, epi));
+                        out[u + 1] = from_f32<T>(activate(v.y, epi));
+                    }
+                    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                        *reinterpret_cast<const uint4 *>(out);
+                }
+                const int col = col0 + p * PIECE;
+                if (by_tma) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && col < N && tm * BM + q * 32 < M) {
+                        tma_store_2d(&mapC, smem_u32(stage), col, tm * BM + q * 32);
+                        bulk_commit_group();
+                    }
+                } else {
+                    __syncwarp();
+                    const int rows = min(32, M - (tm * BM + q * 32));
+                    T *dst = C + (int64_t)(tm * BM + q * 32) * ldc + col;
+                    for (int r = 0; r < rows; ++r, dst += ldc)
+#pragma unroll
+                        for (int e = lane; e < PIECE; e += 32)
+                            if (col + e < N)
+                                dst[e] = *reinterpret_cast<const T *>(stage + r * 128 + ((((e * sizeof(T)) >> 4) ^ (r & 7)) << 4) +
+                                                                      ((e * sizeof(T)) & 15));
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_group0();
+    }
+    if (!ok) {
+        *abort_flag = 1;
+        atomicExch(flags + lonnx::FLAG_TIMEOUT, 8);
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        // copies and MMAs in flight end before shared memory and TMEM go (bounded waits)
+        if (warp == W_MMA && lane == 0) {
+            mma_commit(drained);
+            mbar_wait(drained, 0, nullptr, 400000000ll);
+        }
+        if (warp == W_TMA && lane == 0)
+            for (int i = max(issued - S, 0); i < issued; ++i) mbar_wait(full(i % S), (i / S) & 1, nullptr, 400000000ll);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
     }
 }
 
+// ---- few rows: K split over a cluster ---------------------------------------------
+//
+// One tile of 128 rows of B (the tensor core's rows) x TOK rows of A (its
+// columns) per cluster; each CTA of the cluster takes a run of K's blocks.
+//   warps 0-3  drain: each thread one row of B x TOK sums in registers
+//   warp 4     TMA producer, warp 5 MMA issuer (and TMEM)
+// The CTAs' sums meet in shared memory, TOK / CTAs rows of A to each CTA, added
+// in the CTAs' order.  A thread writes consecutive elements of C's rows with
+// its neighbours, so C needs no alignment.
+constexpr int kSplitThreads = 192;
+template <int TOK>
+struct Split {
+    static constexpr int STAGE = kTile + TOK * KB;
+    static constexpr int TMEM = 2 * TOK < 32 ? 32 : 2 * TOK;
+    static constexpr int SCALES = 4 * 4 * TOK * 4;  // 4 warps x 4 blocks
+    static constexpr int MAX_STAGES = 8 * 18432 / STAGE;
+    static int smem(int stages) {
+        return 1024 + std::max(stages * STAGE, TOK * BM * 4) + SCALES + (2 * MAX_STAGES + 5) * 8 + 8;
+    }
+};
+
+template <int TOK>
+__global__ void __launch_bounds__(kSplitThreads)
+    k_fp8_split(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+                const float *__restrict__ sA, int64_t ldsA, const float *__restrict__ sB, int64_t ldsB,
+                const float *__restrict__ bias, void *__restrict__ C, int dtype, int64_t ldc, int M, int N, int nkb,
+                int stages, int epi, int *flags) {
+    using P = Split<TOK>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    float *sums = reinterpret_cast<float *>(base);  // [TOK][128], over the stages once they are read
+    float *scales = reinterpret_cast<float *>(base + max(stages * P::STAGE, TOK * BM * 4));
+    uint64_t *bar0 = reinterpret_cast<uint64_t *>(scales + 16 * TOK);
+    const uint32_t bars = smem_u32(bar0);
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (P::MAX_STAGES + s); };
+    auto tfull = [&](int b) { return bars + 8 * (2 * P::MAX_STAGES + b); };
+    auto tempty = [&](int b) { return bars + 8 * (2 * P::MAX_STAGES + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * P::MAX_STAGES + 4);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + 2 * P::MAX_STAGES + 5);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + 2 * P::MAX_STAGES + 5) + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    const int tiles_n = (N + BM - 1) / BM;
+    const int tile = blockIdx.x / parts, tm = tile / tiles_n, n0 = (tile - tm * tiles_n) * BM, m0 = tm * TOK;
+    const int b_first = (int)((int64_t)nkb * part / parts), b_last = (int)((int64_t)nkb * (part + 1) / parts);
+    const int blocks = b_last - b_first;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull(b), 1);
+            mbar_init(tempty(b), 4);
+        }
+        mbar_init(drained, 1);
+        fence_mbar_init();
+    }
+    if (warp == 5) {
+        tmem_alloc(smem_u32(tmem_slot), P::TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    bool ok = true;
+    int issued = 0;
+    if (warp == 4) {
+        if (lane == 0) {
+            for (; issued < blocks; ++issued) {
+                const int s = issued % stages;
+                if (!mbar_wait(empty(s), ((issued / stages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                const uint32_t at = smem_u32(base + s * P::STAGE);
+                mbar_arrive_expect_tx(full(s), P::STAGE);
+                tma_load_2d(at, &mapB, full(s), (b_first + issued) * KB, n0);
+                tma_load_2d(at + kTile, &mapA, full(s), (b_first + issued) * KB, m0);
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(BM, TOK);
+            for (int j = 0; j < blocks; ++j) {
+                const int s = j % stages, buf = j & 1;
+                if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                if (!mbar_wait(full(s), (j / stages) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t da = smem_desc_sw128(smem_u32(base + s * P::STAGE));
+                const uint64_t db = smem_desc_sw128(smem_u32(base + s * P::STAGE + kTile));
+#pragma unroll
+                for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * TOK, da + 2 * k, db + 2 * k, idesc, k > 0);
+                mma_commit(empty(s));
+                mma_commit(tfull(buf));
+            }
+        }
+    } else {
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        constexpr int PER = (TOK + 31) / 32;  // rows of A whose scales a lane fetches
+        float *my = scales + warp * 4 * TOK;  // [4 blocks][TOK], this warp's copy
+        const float *rb = sB + (int64_t)(n0 / KB) * ldsB;
+        uint64_t acc[TOK / 2];
+#pragma unroll
+        for (int i = 0; i < TOK / 2; ++i) acc[i] = 0;
+        float na[PER][4], nb[4];
+        auto fetch = [&](int b) {
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                const int m = m0 + lane + 32 * p;
+                const bool valid = m < M && lane + 32 * p < TOK;
+                load_scales(na[p], sA + (int64_t)(valid ? m : 0) * ldsA, b, b_last, valid);
+            }
+            load_scales(nb, rb, b, b_last, true);
+        };
+        fetch(b_first);
+        for (int b0 = 0; b0 < blocks && ok; b0 += 4) {
+            __syncwarp();
+#pragma unroll
+            for (int p = 0; p < PER; ++p)
+                if (lane + 32 * p < TOK)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) my[i * TOK + lane + 32 * p] = na[p][i] * nb[i];
+            __syncwarp();
+            fetch(b_first + b0 + 4);
+            for (int i = 0; i < 4 && b0 + i < blocks; ++i) {
+                const int j = b0 + i, buf = j & 1;
+                // (one answer for the warp: its next steps are collective)
+                    if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
+                tc_fence_after();
+                constexpr int CH = TOK < 32 ? TOK : 32;
+#pragma unroll
+                for (int c = 0; c < TOK / CH; ++c) {
+                    uint32_t r[CH];
+                    if constexpr (CH == 16) tmem_ld_32x32b_x16(lanes + buf * TOK + c * CH, r);
+                    else tmem_ld_32x32b_x32(lanes + buf * TOK + c * CH, r);
+                    tmem_ld_wait();
+                    if (c == TOK / CH - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(tempty(buf));
+                    }
+                    const ulonglong2 *s4 = reinterpret_cast<const ulonglong2 *>(my + i * TOK + c * CH);
+#pragma unroll
+                    for (int u = 0; u < CH / 4; ++u) {
+                        const ulonglong2 s = s4[u];
+                        fma2(acc[c * (CH / 2) + 2 * u], pack2u(r[4 * u], r[4 * u + 1]), s.x);
+                        fma2(acc[c * (CH / 2) + 2 * u + 1], pack2u(r[4 * u + 2], r[4 * u + 3]), s.y);
+                    }
+                }
+            }
+        }
+        // the last block's MMAs have read the stages: the sums may go over them
+        if (ok) {
+#pragma unroll
+            for (int i = 0; i < TOK / 2; ++i) {
+                const float2 v = unpack2(acc[i]);
+                sums[(2 * i) * BM + threadIdx.x] = v.x;
+                sums[(2 * i + 1) * BM + threadIdx.x] = v.y;
+            }
+        }
+    }
+    if (!ok) {
+        *abort_flag = 1;
+        atomicExch(flags + lonnx::FLAG_TIMEOUT, 9);
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        if (warp == 5 && lane == 0) {
+            mma_commit(drained);
+            mbar_wait(drained, 0, nullptr, 400000000ll);
+        }
+        if (warp == 4 && lane == 0)
+            for (int i = max(issued - stages, 0); i < issued; ++i)
+                mbar_wait(full(i % stages), (i / stages) & 1, nullptr, 400000000ll);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) {
+        // before the cluster's barrier: a CTA never holds TMEM while it waits for another CTA
+        tc_fence_after();
+        tmem_dealloc(tmem, P::TMEM);
+    }
+    if (parts > 1) cluster.sync();
+    if (threadIdx.x < BM) {
+        const int n = n0 + threadIdx.x;
+        const int first = TOK * part / parts, last = min(TOK * (part + 1) / parts, M - m0);
+        const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
+        for (int m = first; m < last; ++m) {
+            float v = 0.0f;
+            for (int p = 0; p < parts; ++p) v += cluster.map_shared_rank(sums, p)[m * BM + threadIdx.x];
+            if (n < N) {
+                v = activate(v + bv, epi);
+                const int64_t at = (int64_t)(m0 + m) * ldc + n;
+                if (dtype == LONNX_DT_F32) static_cast<float *>(C)[at] = v;
+                else if (dtype == LONNX_DT_F16) static_cast<__half *>(C)[at] = from_f32<__half>(v);
+                else static_cast<__nv_bfloat16 *>(C)[at] = from_f32<__nv_bfloat16>(v);
+            }
+        }
+    }
+    if (parts > 1) cluster.sync();  // the others' shared memory is read until here
+}
+
+// K = 0: the bias through the activation
 template <typename T>
-int gemm_fp8(lonnx_ctx *ctx, const uint8_t *A, int64_t lda, const float *sA, int64_t ldsA, const uint8_t *B,
-             int64_t ldb, const float *sB, int64_t ldsB, const float *bias, void *C, int64_t ldc, int M, int N, int K,
-             int epi) {
-    const dim3 grid((N + 15) / 16, (M + 15) / 16);
-    k_gemm_fp8_plain<T><<<grid, 256, 0, ctx->stream>>>(A, lda, sA, ldsA, B, ldb, sB, ldsB, bias, static_cast<T *>(C),
-                                                      ldc, M, N, K, epi);
+__global__ void k_fp8_no_columns(const float *__restrict__ bias, T *__restrict__ C, int64_t ldc, int M, int N, int epi) {
+    const int64_t total = (int64_t)M * N, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int64_t m = i / N, n = i - m * N;
+        C[m * ldc + n] = from_f32<T>(activate(bias ? bias[n] : 0.0f, epi));
+    }
+}
+
+// ---- host side ------------------------------------------------------------------
+
+// row-major [rows, cols] of es-byte elements, leading dimension ld elements, box of 128 bytes x box_rows
+int tile_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int es, int64_t rows, int64_t cols,
+             int64_t ld, int box_rows) {
+    lonnx::tc::EncodeTiledFn enc = lonnx::tc::encode_tiled();
+    if (!enc) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LONNX_OK;
+}
+
+struct Problem {
+    const uint8_t *A, *B;
+    const float *sA, *sB, *bias;
+    void *C;
+    int64_t lda, ldb, ldsA, ldsB, ldc;
+    int dtype, M, N, K, epi;
+};
+
+template <int BN, typename T>
+int launch_wide(lonnx_ctx *ctx, const Problem &p) {
+    using W = Wide<BN>;
+    CUtensorMap ma, mb, mc;
+    int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, BM);
+    if (!rc) rc = tile_map(&mb, p.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.ldb, BN);
+    if (rc) return rc;
+    const bool by_tma = ((uintptr_t)p.C & 15) == 0 && p.ldc * (int64_t)sizeof(T) % 16 == 0;
+    mc = ma;  // unused unless by_tma
+    if (by_tma) {
+        const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : p.dtype == LONNX_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        rc = tile_map(&mc, p.C, type, (int)sizeof(T), p.M, p.N, p.ldc, 32);
+        if (rc) return rc;
+    }
+    const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+    if (tiles >= (1ll << 31) - 1024) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
+    auto kernel = k_fp8_wide<BN, T>;
+    LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM));
+    kernel<<<(unsigned)std::min<int64_t>(tiles, ctx->num_sms), kWideThreads, W::SMEM, ctx->stream>>>(
+        ma, mb, mc, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, static_cast<T *>(p.C), p.ldc, p.M, p.N, (p.K + KB - 1) / KB,
+        p.epi, by_tma, ctx->dev_flags);
     LONNX_CHECK_LAUNCH(ctx);
     return LONNX_OK;
+}
+
+template <int TOK>
+int launch_split(lonnx_ctx *ctx, const Problem &p) {
+    using P = Split<TOK>;
+    CUtensorMap ma, mb;
+    int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, TOK);
+    if (!rc) rc = tile_map(&mb, p.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.ldb, BM);
+    if (rc) return rc;
+    const int nkb = (p.K + KB - 1) / KB;
+    const int64_t tiles = (int64_t)((p.N + BM - 1) / BM) * ((p.M + TOK - 1) / TOK);
+    if (tiles > (1 << 27)) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= 2 * ctx->num_sms && nkb >= parts * 4) parts *= 2;
+    const int stages = std::min((nkb + parts - 1) / parts, P::MAX_STAGES), smem = P::smem(stages);
+    auto kernel = k_fp8_split<TOK>;
+    LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * parts));
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ctx->launches++;
+    LONNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, p.C, p.dtype, p.ldc, p.M,
+                                  p.N, nkb, stages, p.epi, ctx->dev_flags));
+    return LONNX_OK;
+}
+
+template <typename T>
+int launch(lonnx_ctx *ctx, const Problem &p) {
+    if (p.K == 0) {
+        const int64_t total = (int64_t)p.M * p.N;
+        k_fp8_no_columns<T><<<(unsigned)std::min<int64_t>((total + 255) / 256, ctx->num_sms * 16), 256, 0, ctx->stream>>>(
+            p.bias, static_cast<T *>(p.C), p.ldc, p.M, p.N, p.epi);
+        LONNX_CHECK_LAUNCH(ctx);
+        return LONNX_OK;
+    }
+    const int64_t tm = (p.M + BM - 1) / BM;
+    if (p.M <= 16) return launch_split<16>(ctx, p);
+    if (p.M <= 32) return launch_split<32>(ctx, p);
+    if (p.M <= 64) return launch_split<64>(ctx, p);
+    if (tm * ((p.N + 255) / 256) >= ctx->num_sms) return launch_wide<256, T>(ctx, p);
+    if (tm * ((p.N + 127) / 128) >= ctx->num_sms) return launch_wide<128, T>(ctx, p);
+    return launch_split<128>(ctx, p);
 }
 
 }  // namespace
@@ -84,7 +650,7 @@ extern "C" LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t l
     if (M < 0 || N < 0 || K < 0) return set_error(LONNX_E_BADARG, "gemm_fp8: negative size");
     if (epilogue < LONNX_EPI_NONE || epilogue > LONNX_EPI_GELU_ERF)
         return set_error(LONNX_E_BADARG, "gemm_fp8: epilogue %d", epilogue);
-    if (lda < K || ldb < K || ldc < N || ldsA < (K + KB - 1) / KB || ldsB < (K + KB - 1) / KB)
+    if (lda < K || ldb < K || ldc < N || ldsA < ((int64_t)K + KB - 1) / KB || ldsB < ((int64_t)K + KB - 1) / KB)
         return set_error(LONNX_E_SHAPE, "gemm_fp8: a leading dimension is smaller than its row");
     if (((uintptr_t)A & 15) || ((uintptr_t)B & 15) || lda % 16 || ldb % 16)
         return set_error(LONNX_E_BADARG, "gemm_fp8: rows of A and B must start on 16 bytes (pointers and leading dimensions)");
@@ -94,10 +660,9 @@ extern "C" LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t l
     if (rc) return rc;
     if (M == 0 || N == 0) return LONNX_OK;
     if (!C || (K > 0 && (!A || !B || !scaleA || !scaleB))) return set_error(LONNX_E_BADARG, "gemm_fp8: null pointer");
-    const uint8_t *a = static_cast<const uint8_t *>(A), *b = static_cast<const uint8_t *>(B);
-    if (dtypeC == LONNX_DT_F32)
-        return gemm_fp8<float>(ctx, a, lda, scaleA, ldsA, b, ldb, scaleB, ldsB, bias, C, ldc, M, N, K, epilogue);
-    if (dtypeC == LONNX_DT_F16)
-        return gemm_fp8<__half>(ctx, a, lda, scaleA, ldsA, b, ldb, scaleB, ldsB, bias, C, ldc, M, N, K, epilogue);
-    return gemm_fp8<__nv_bfloat16>(ctx, a, lda, scaleA, ldsA, b, ldb, scaleB, ldsB, bias, C, ldc, M, N, K, epilogue);
+    const Problem p{static_cast<const uint8_t *>(A), static_cast<const uint8_t *>(B), scaleA, scaleB, bias, C,
+                    lda, ldb, ldsA, ldsB, ldc, dtypeC, M, N, K, epilogue};
+    if (dtypeC == LONNX_DT_F32) return launch<float>(ctx, p);
+    if (dtypeC == LONNX_DT_F16) return launch<__half>(ctx, p);
+    return launch<__nv_bfloat16>(ctx, p);
 }

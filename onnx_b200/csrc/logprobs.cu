@@ -107,19 +107,22 @@ template <bool TOP>
 struct Warp {
     Softmax a;       // m is the same in every lane, s and w are the lane's
     uint64_t list;   // lane's entry of the descending list
-    float thr;       // value of the k-th entry; NaN while there are fewer
+    uint64_t kth;    // the k-th entry; 0 while there are fewer
+    float thr;       // its value, NaN while there are fewer
     float c;
     int k;
 
     __device__ __forceinline__ void reset(float c_, int k_) {
         a = {-FLT_MAX, 0.0f, 0.0f};
         list = 0;
+        kth = 0;
         thr = __uint_as_float(0x7fc00000u);
         c = c_;
         k = k_;
     }
     __device__ __forceinline__ void set_thr() {
-        const uint32_t o = (uint32_t)(__shfl_sync(kAll, list, k - 1) >> 32);
+        kth = __shfl_sync(kAll, list, k - 1);
+        const uint32_t o = (uint32_t)(kth >> 32);
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
     }
     __device__ __forceinline__ void insert(uint64_t key, int lane) {
@@ -160,14 +163,8 @@ struct Warp {
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    // >= where the index may be lower than that of an equal entry
-                    bool want = valid(j) && !(x[j] < thr);
-                    uint64_t key = 0;
-                    if (want) {
-                        key = make_key(x[j], idx(j));
-                        want = key != mine;
-                    }
-                    unsigned todo = __ballot_sync(kAll, want);
+                    const uint64_t key = make_key(x[j], idx(j));
+                    unsigned todo = __ballot_sync(kAll, valid(j) && key > kth && key != mine);
                     while (todo) {
                         const int src = __ffs(todo) - 1;
                         todo &= todo - 1;
