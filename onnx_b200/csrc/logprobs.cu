@@ -8,22 +8,30 @@
 //   values are equal
 //
 // in one pass over the row: a running maximum m with S and W rescaled when it
-// grows, and a sorted list of the k best per warp.  All sums are fp32; a
-// thread adds at most vocab / 256 terms, the rest is a tree.  x - m is taken
-// before any scaling, so logits of the type's lowest value stay ordinary
-// numbers; -inf adds exactly zero.
+// grows, and a sorted list of the k best groups of elements per warp.  All sums
+// are fp32; a thread adds at most vocab / 256 terms, the rest is a tree.  x - m
+// is taken before any scaling, so logits of the type's lowest value stay
+// ordinary numbers; -inf adds exactly zero.
 //
-// Bound by HBM (each logit is read once, 16 bytes a thread and load).  Per
-// element it issues about a load's share, a subtraction, a multiplication, a
-// base-2 exponential, a clamp, a sum and an FMA; the list costs one comparison
-// of 16 or 32 elements' maximum with the k-th best, and an insertion about
-// k (1 + ln(vocab / k)) times a row.
+// The alternatives.  A group is what one lane loads at once, 64 bytes of a row;
+// its key is its best element under (value, lowest index first).  The k best
+// elements lie in the k groups of the best keys, so the scan lists groups, with
+// one comparison per 64 bytes and lane, and the elements of the k listed groups
+// are read again at the end.  (A list of elements took a comparison each and
+// four times the insertions: at one row of 250037 floats and k = 20 it made
+// the kernel 32 us instead of 10.)
+//
+// Bound by HBM (each logit is read once, 16 bytes a thread and load, the next
+// 64 bytes in flight while the last are summed).  Pairs of elements share their
+// additions, multiplications and FMAs (f32x2); per element that leaves about
+// 5 instructions and one base-2 exponential.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "lonnx_internal.cuh"
 
@@ -58,15 +66,43 @@ __device__ __forceinline__ float unordered(uint32_t o) {
 // (value, lowest index first) as one number; 0 is "no entry"
 __device__ __forceinline__ uint64_t make_key(float v, uint32_t idx) { return (uint64_t)ordered(v) << 32 | (uint32_t)~idx; }
 
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// With t = (x - m) c, c = log2(e) / T: s = sum of 2^t, w = sum of t 2^t
 struct Softmax {
-    float m, s, w;  // w: sum of (x - m) e^((x - m) / T)
+    float m, s, w;
 };
 
-// b's sums added to a's, both to the larger maximum; c = log2(e) / T
+// a's sums to a larger maximum
 __device__ __forceinline__ void rescale(Softmax &a, float m, float c) {
-    const float d = a.m - m, f = ex2(d * c);
-    // f == 0: the old terms vanish (d may be -inf there); * 0 keeps a NaN
-    a.w = f == 0.0f ? a.w * 0.0f : f * fmaf(a.s, d, a.w);
+    const float t = (a.m - m) * c, f = ex2(t);
+    // f == 0: the old terms vanish (t may be -inf there); * 0 keeps a NaN
+    a.w = f == 0.0f ? a.w * 0.0f : f * fmaf(a.s, t, a.w);
     a.s *= f;
     a.m = m;
 }
@@ -105,17 +141,17 @@ __device__ __forceinline__ uint64_t merge_desc(uint64_t a, uint64_t b, int lane)
 // What a warp has seen of its row.
 template <bool TOP>
 struct Warp {
-    Softmax a;       // m is the same in every lane, s and w are the lane's
-    uint64_t list;   // lane's entry of the descending list
-    uint64_t kth;    // the k-th entry; 0 while there are fewer
-    float thr;       // its value, NaN while there are fewer
+    float m;            // running maximum, the same in every lane
+    uint64_t s2, w2;    // the lane's sums, in two halves
+    uint64_t list;      // lane's entry of the descending list of groups
+    uint64_t kth;       // the k-th entry; 0 while there are fewer
+    float thr;          // its value, NaN while there are fewer
     float c;
     int k;
 
     __device__ __forceinline__ void reset(float c_, int k_) {
-        a = {-FLT_MAX, 0.0f, 0.0f};
-        list = 0;
-        kth = 0;
+        m = -FLT_MAX;
+        s2 = w2 = list = kth = 0;
         thr = __uint_as_float(0x7fc00000u);
         c = c_;
         k = k_;
@@ -125,58 +161,123 @@ struct Warp {
         const uint32_t o = (uint32_t)(kth >> 32);
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
     }
-    __device__ __forceinline__ void insert(uint64_t key, int lane) {
-        const int p = __popc(__ballot_sync(kAll, list > key));
-        if (p >= k) return;
-        const uint64_t up = __shfl_up_sync(kAll, list, 1);
-        list = lane < p ? list : lane == p ? key : up;
+    // keys of lanes in `todo` into the list
+    __device__ __forceinline__ void insert(uint64_t key, unsigned todo, int lane) {
+        if (__popc(todo) > 6) {
+            // (sorting and merging cost about as much as 6 single insertions)
+            list = merge_desc(list, sort_desc(todo >> lane & 1 ? key : 0, lane), lane);
+        } else {
+            while (todo) {
+                const int src = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const uint64_t one = __shfl_sync(kAll, key, src);
+                const int p = __popc(__ballot_sync(kAll, list > one));
+                const uint64_t up = __shfl_up_sync(kAll, list, 1);
+                list = lane < p ? list : lane == p ? one : up;
+            }
+        }
         set_thr();
     }
-    __device__ __forceinline__ void add(float x) {
-        const float d = x - a.m, e = ex2(d * c);
-        a.s += e;
-        a.w = fmaf(e, fmaxf(d, -FLT_MAX), a.w);  // d = -inf: e = 0, and 0 * -inf would be NaN
+    __device__ __forceinline__ void raise(float best, int lane) {
+        float top = best;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+        if (!(top > m)) return;
+        const float2 s = unpack2(s2), w = unpack2(w2);
+        Softmax a{m, s.x, w.x}, b{m, s.y, w.y};
+        rescale(a, top, c);
+        rescale(b, top, c);
+        s2 = pack2(a.s, b.s);
+        w2 = pack2(a.w, b.w);
+        m = top;
     }
-    // N values a lane; value j has index idx(j), or is not there (valid(j) false)
+    __device__ __forceinline__ void add(float x, float y) {
+        const uint64_t t = mul2(add2(pack2(x, y), pack2(-m, -m)), pack2(c, c));
+        const float2 u = unpack2(t);
+        // -inf: 2^t = 0, and 0 * -inf would be NaN; a NaN stays in s
+        const uint64_t e = pack2(ex2(u.x), ex2(u.y));
+        s2 = add2(s2, e);
+        w2 = fma2(e, pack2(fmaxf(u.x, -FLT_MAX), fmaxf(u.y, -FLT_MAX)), w2);
+    }
+    // N values a lane, in order of their indices idx(j); those past the row's end
+    // (valid(j) false, the first never before others) are -inf
     template <int N, typename Idx, typename Valid>
-    __device__ __forceinline__ void take(const float (&x)[N], float best, bool first, int lane, const int *shared_thr,
-                                         Idx idx, Valid valid) {
-        bool slow = best > a.m;
-        if (TOP && !(best <= thr))
-            slow |= !shared_thr || !(best < unordered((uint32_t)*(volatile const int *)shared_thr));
-        if (__any_sync(kAll, slow)) {
-            float top = best;
+    __device__ __forceinline__ void take(const float (&x)[N], int lane, const int *shared_thr, Idx idx, Valid valid) {
+        float best = -INFINITY;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-            if (top > a.m) rescale(a, top, c);
+        for (int j = 0; j < N; ++j) best = fmaxf(best, x[j]);
+        // a group can enter the list if it is above the k-th of this warp's, and
+        // not below that of another warp of the CTA
+        bool enters = false;
+        if (TOP) enters = valid(0) && !(best <= thr) && !(shared_thr && best < unordered((uint32_t)*(volatile const int *)shared_thr));
+        if (__any_sync(kAll, enters || best > m)) {
+            raise(best, lane);
             if constexpr (TOP) {
-                uint64_t mine = 0;
-                if (first) {
-                    // the lanes' best values, sorted, are the first list
+                unsigned todo = __ballot_sync(kAll, enters);
+                if (todo) {
+                    uint32_t at = idx(0);
+                    bool any = false;
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const uint64_t key = valid(j) ? make_key(x[j], idx(j)) : 0;
-                        mine = key > mine ? key : mine;
-                    }
-                    list = sort_desc(mine, lane);
-                    set_thr();
-                }
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const uint64_t key = make_key(x[j], idx(j));
-                    unsigned todo = __ballot_sync(kAll, valid(j) && key > kth && key != mine);
-                    while (todo) {
-                        const int src = __ffs(todo) - 1;
-                        todo &= todo - 1;
-                        insert(__shfl_sync(kAll, key, src), lane);
-                    }
+                    for (int j = N - 1; j >= 0; --j)
+                        if (x[j] == best && valid(j)) {
+                            at = idx(j);
+                            any = true;
+                        }
+                    const uint64_t key = make_key(any ? best : __uint_as_float(0x7fc00000u), at);
+                    insert(key, todo, lane);
                 }
             }
         }
+        if constexpr (N == 1) {
+            add(x[0], -INFINITY);
+        } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (valid(j)) add(x[j]);
+            for (int j = 0; j < N; j += 2) add(x[j], x[j + 1]);
+        }
     }
+    // the warp's sums, the same in every lane
+    __device__ __forceinline__ Softmax total() const {
+        const float2 s = unpack2(s2), w = unpack2(w2);
+        Softmax a{m, s.x + s.y, w.x + w.y};
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a.s += __shfl_xor_sync(kAll, a.s, o);
+            a.w += __shfl_xor_sync(kAll, a.w, o);
+        }
+        return a;
+    }
+};
+
+// A row's vectors: 16-byte ones from the first aligned element, the elements
+// before and after them (under 16 bytes each).  Groups are U vectors, 32 apart,
+// of a chunk of 32 * U.
+template <typename T>
+struct Row {
+    static constexpr int VN = 16 / (int)sizeof(T);
+    const T *x;
+    const uint4 *v;
+    uint32_t vocab, head, nvec, tail;
+    __device__ __forceinline__ Row(const T *x_, uint32_t vocab_) : x(x_), vocab(vocab_) {
+        head = min(vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
+        nvec = (vocab - head) / VN;
+        tail = vocab - head - nvec * VN;
+        v = reinterpret_cast<const uint4 *>(x + head);
+    }
+    // vectors at + 32 u, -inf past the end
+    __device__ __forceinline__ void load(uint4 (&r)[U], uint32_t at) const {
+        const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = at + 32 * u < nvec ? __ldcs(v + at + 32 * u) : make_uint4(inf, inf, inf, inf);
+    }
+    static __device__ __forceinline__ void unpack(const uint4 (&r)[U], float (&f)[U * VN]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const T *p = reinterpret_cast<const T *>(&r[u]);
+#pragma unroll
+            for (int j = 0; j < VN; ++j) f[u * VN + j] = to_f32(p[j]);
+        }
+    }
+    __device__ __forceinline__ uint32_t index(uint32_t at, int j) const { return head + (at + 32 * (j / VN)) * VN + j % VN; }
 };
 
 struct Args {
@@ -191,10 +292,12 @@ struct Args {
     int *flags;
 };
 
-// The row's answer from its sums and list: one warp, every lane with the same `a`.
+// The row's answer from its sums and list of groups: one warp, every lane with
+// the same `a`.
 template <typename T, bool TOP>
-__device__ __forceinline__ void finish(const Args &g, const T *xr, int64_t row, const Softmax &a, uint64_t list,
+__device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t row, const Softmax &a, Warp<TOP> &st,
                                        int lane) {
+    constexpr int N = U * Row<T>::VN;
     const bool none = a.s == 0.0f;  // every logit -inf: no token has any probability
     const float log_s = logf(a.s);
     if (lane == 0) {
@@ -202,18 +305,36 @@ __device__ __forceinline__ void finish(const Args &g, const T *xr, int64_t row, 
             const int64_t t = g.targets[row];
             float lp = __uint_as_float(0x7fc00000u);
             if (t < (int64_t)g.vocab)
-                lp = none ? -INFINITY : fmaf(to_f32(xr[t]) - a.m, g.inv_t, -log_s);
+                lp = none ? -INFINITY : fmaf(to_f32(r.x[t]) - a.m, g.inv_t, -log_s);
             else
                 atomicExch(g.flags + lonnx::FLAG_TARGET, 1);
             g.logprob[row] = lp;
         }
-        if (g.entropy) g.entropy[row] = none ? 0.0f : log_s - a.w / a.s * g.inv_t;
+        if (g.entropy) g.entropy[row] = none ? 0.0f : fmaf(a.w / a.s, -0.69314718055994530942f, log_s);
     }
     if constexpr (TOP) {
+        // the listed groups' other elements; an element outside the vectors is a group of its own
+        const uint64_t mine = st.list;
+        const uint32_t i = ~(uint32_t)mine - r.head, vec = i / Row<T>::VN;
+        const bool group = lane < g.k && mine && ~(uint32_t)mine >= r.head && vec < r.nvec;
+        const uint32_t at = vec / (32 * U) * (32 * U) + vec % 32;
+        uint4 raw[U];
+        r.load(raw, group ? at : r.nvec);
+        float x[N];
+        Row<T>::unpack(raw, x);
+        st.set_thr();
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t idx = r.index(at, j);
+            const uint64_t key = make_key(x[j], idx);
+            const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
+            const unsigned todo = __ballot_sync(kAll, want);
+            if (todo) st.insert(key, todo, lane);
+        }
         if (lane < g.k) {
-            g.top_id[row * g.k + lane] = (int64_t)(uint32_t)~(uint32_t)list;
+            g.top_id[row * g.k + lane] = (int64_t)(uint32_t)~(uint32_t)st.list;
             g.top_logprob[row * g.k + lane] =
-                none ? -INFINITY : fmaf(unordered((uint32_t)(list >> 32)) - a.m, g.inv_t, -log_s);
+                none ? -INFINITY : fmaf(unordered((uint32_t)(st.list >> 32)) - a.m, g.inv_t, -log_s);
         }
     }
 }
@@ -233,49 +354,31 @@ __device__ __forceinline__ void finish_padding(const Args &g, int64_t row, int l
         }
 }
 
-// Warp `w` of `nw` over one row: 16-byte vectors from the row's first aligned
-// one in chunks of 32 * U, chunk i to warp i % nw; the elements before and
-// after them (under 16 bytes each) to the last warp, one a lane.
+// Warp `w` of `nw` over one row: chunk i to warp i % nw, the elements outside
+// the vectors to the last warp, one a lane.
 template <typename T, bool TOP>
-__device__ __forceinline__ void scan(Warp<TOP> &st, const T *xr, uint32_t vocab, int w, int nw, int lane,
-                                     int *shared_thr) {
-    constexpr int VN = 16 / (int)sizeof(T);
-    const uint32_t head = min(vocab, (uint32_t)((16 - ((uintptr_t)xr & 15)) & 15) / (uint32_t)sizeof(T));
-    const uint32_t nvec = (vocab - head) / VN, tail = vocab - head - nvec * VN;
-    const uint4 *xv = reinterpret_cast<const uint4 *>(xr + head);
-    bool first = true;
-    for (uint32_t v0 = w * 32 * U; v0 < nvec; v0 += nw * 32 * U) {
-        uint4 raw[U];
+__device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, int *shared_thr) {
+    const uint32_t step = nw * 32 * U;
+    uint32_t v0 = w * 32 * U;
+    uint4 next[U];
+    if (v0 < r.nvec) r.load(next, v0 + lane);
+    while (v0 < r.nvec) {
         const uint32_t at = v0 + lane;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (at + 32 * u < nvec) raw[u] = __ldcs(xv + at + 32 * u);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (v0 + 32 * u >= nvec) break;
-            const bool in = at + 32 * u < nvec;
-            float x[VN];
-            const T *p = reinterpret_cast<const T *>(&raw[u]);
-            float best = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < VN; ++j) {
-                x[j] = in ? to_f32(p[j]) : -INFINITY;
-                best = fmaxf(best, x[j]);
-            }
-            const uint32_t i0 = head + (at + 32 * u) * VN;
-            st.take(x, best, first, lane, shared_thr, [&](int j) { return i0 + j; }, [&](int) { return in; });
-            first = false;
-        }
+        float x[U * Row<T>::VN];
+        Row<T>::unpack(next, x);
+        v0 += step;
+        if (v0 < r.nvec) r.load(next, v0 + lane);
+        st.take(x, lane, shared_thr, [&](int j) { return r.index(at, j); },
+                [&](int j) { return at + 32 * (j / Row<T>::VN) < r.nvec; });
         if (TOP && shared_thr && lane == 0 && st.thr == st.thr) atomicMax((unsigned *)shared_thr, ordered(st.thr));
     }
-    if (w == nw - 1 && head + tail) {
-        const bool in = lane < head || (lane >= 16 && lane - 16 < tail);
-        const uint32_t idx = lane < 16 ? lane : head + nvec * VN + lane - 16;
-        float x[1] = {in ? to_f32(xr[idx]) : -INFINITY};
-        // the head's indices are below the list's: no shortcut for equal values
-        const float thr = st.thr;
-        if (TOP && in && x[0] == thr) st.thr = __uint_as_float(0x7fc00000u);
-        st.take(x, x[0], first, lane, nullptr, [&](int) { return idx; }, [&](int) { return in; });
+    if (w == nw - 1 && r.head + r.tail) {
+        const bool in = lane < r.head || (lane >= 16 && lane - 16 < r.tail);
+        const uint32_t idx = lane < 16 ? lane : r.head + r.nvec * Row<T>::VN + lane - 16;
+        const float x[1] = {in ? to_f32(r.x[idx]) : -INFINITY};
+        // the head's indices are below the list's: equal values enter, too
+        if (TOP && in && x[0] == st.thr) st.thr = __uint_as_float(0x7fc00000u);
+        st.take(x, lane, nullptr, [&](int) { return idx; }, [&](int) { return in; });
     }
 }
 
@@ -288,17 +391,12 @@ __global__ void __launch_bounds__(256) k_logprobs_warp(const T *__restrict__ x, 
             finish_padding<TOP>(g, row, lane);
             continue;
         }
-        const T *xr = x + row * g.ld;
+        const Row<T> r(x + row * g.ld, g.vocab);
         const float c = g.inv_t * 1.44269504088896340736f;
         Warp<TOP> st;
         st.reset(c, g.k);
-        scan<T, TOP>(st, xr, g.vocab, 0, 1, lane, nullptr);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            st.a.s += __shfl_xor_sync(kAll, st.a.s, o);
-            st.a.w += __shfl_xor_sync(kAll, st.a.w, o);
-        }
-        finish<T, TOP>(g, xr, row, st.a, st.list, lane);
+        scan<T, TOP>(st, r, 0, 1, lane, nullptr);
+        finish<T, TOP>(g, r, row, st.total(), st, lane);
     }
 }
 
@@ -322,28 +420,24 @@ __global__ void __launch_bounds__(256) k_logprobs_cta(const T *__restrict__ x, A
             if (part == 0 && w == 0) finish_padding<TOP>(g, row, lane);
             continue;
         }
-        const T *xr = x + row * g.ld;
+        const Row<T> r(x + row * g.ld, g.vocab);
         if (threadIdx.x == 0) thr = 0;
         __syncthreads();
         Warp<TOP> st;
         st.reset(c, g.k);
-        scan<T, TOP>(st, xr, g.vocab, part * NW + w, parts * NW, lane, &thr);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            st.a.s += __shfl_xor_sync(kAll, st.a.s, o);
-            st.a.w += __shfl_xor_sync(kAll, st.a.w, o);
-        }
-        if (lane == 0) sums[w] = st.a;
+        scan<T, TOP>(st, r, part * NW + w, parts * NW, lane, &thr);
+        Softmax a = st.total();
+        if (lane == 0) sums[w] = a;
         if constexpr (TOP) lists[w][lane] = st.list;
         __syncthreads();
         if (w == 0) {
 #pragma unroll
             for (int i = 1; i < NW; ++i) {
-                join(st.a, sums[i], c);
+                join(a, sums[i], c);
                 if constexpr (TOP) st.list = merge_desc(st.list, lists[i][lane], lane);
             }
             if (parts > 1) {
-                if (lane == 0) cta_sums = st.a;
+                if (lane == 0) cta_sums = a;
                 if constexpr (TOP) cta_list[lane] = st.list;
             }
         }
@@ -351,7 +445,7 @@ __global__ void __launch_bounds__(256) k_logprobs_cta(const T *__restrict__ x, A
             cluster.sync();
             if (part == 0 && w == 0) {
                 for (int i = 1; i < parts; ++i) {
-                    join(st.a, *cluster.map_shared_rank(&cta_sums, i), c);
+                    join(a, *cluster.map_shared_rank(&cta_sums, i), c);
                     if constexpr (TOP) st.list = merge_desc(st.list, cluster.map_shared_rank(cta_list, i)[lane], lane);
                 }
             }
@@ -359,7 +453,7 @@ __global__ void __launch_bounds__(256) k_logprobs_cta(const T *__restrict__ x, A
         } else {
             __syncthreads();
         }
-        if (part == 0 && w == 0) finish<T, TOP>(g, xr, row, st.a, st.list, lane);
+        if (part == 0 && w == 0) finish<T, TOP>(g, r, row, a, st, lane);
     }
 }
 

@@ -403,9 +403,10 @@ def test_logprobs_padding_rows(tctx, vocab):
     assert (got["top_id"][pad] == -1).all() and (got["top_logprob"][pad] == float("-inf")).all()
     want, z = scores_reference(x[~pad], target[~pad], 3, 1.0)
     check_scores({n: t[~pad] for n, t in got.items()}, want, z, vocab, 1.0)
-    # without targets every row is scored
+    # without targets every row is scored; these rows start on other addresses, and the order of a
+    # row's sums goes by its first 16-byte boundary, so the two agree within the bounds, not in bits
     bare = run_scores(tctx, x[~pad], None, 3)
-    assert torch.equal(bare["entropy"], got["entropy"][~pad]) and torch.equal(bare["top_id"], got["top_id"][~pad])
+    check_scores({**bare, "logprob": got["logprob"][~pad]}, want, z, vocab, 1.0)
 
 
 @pytest.mark.parametrize("vocab", [700, 12345])
