@@ -91,22 +91,30 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 
 // ---- wide tiles -----------------------------------------------------------------
 //
-// CTA = 10 warps, one per SM, walking tiles of 128 x BN:
-//   warps 0-7  drain: each thread one row x BN / 2 columns in registers; then
-//              the epilogue, 128 bytes of a row at a time through 4 KB of
-//              shared memory per warp and out by TMA (or, where rows of C do
-//              not start on 16 bytes, by coalesced element stores)
-//   warp 8     TMA producer, warp 9 MMA issuer (and TMEM)
+// CTA = 20 warps, one per SM, walking tiles of 128 x BN:
+//   warps 0-15   drain: each thread one row x BN / 4 columns in registers (four
+//                warps a scheduler: the TMEM loads of one hide behind the FMAs
+//                of the others); then the epilogue, 64 bytes of a row at a time
+//                through 2 KB of shared memory per warp and out by TMA (or,
+//                where rows of C do not start on 16 bytes, by element stores
+//                that coalesce along rows)
+//   warp 16      TMA producer, warp 17 MMA issuer (and TMEM)
+//   warps 18, 19 the block's scales: sA[m, b] * sB[n / 128, b] of the tile's 128
+//                rows and BN / 128 column blocks into shared memory, one slot
+//                per TMEM buffer, under the same barriers
+// The drain warps take registers from the other four (setmaxnreg): 512 x 112 +
+// 128 x 32 = 640 x 96, the launch's.
 template <int BN>
 struct Wide {
     static constexpr int STAGE = kTile + BN * KB;
     static constexpr int S = BN == 256 ? 4 : 6;
-    static constexpr int STAGING = 8 * 4096;
-    static constexpr int SMEM = 1024 + S * STAGE + STAGING + (2 * S + 5) * 8 + 8;
+    static constexpr int STAGING = 16 * 2048;
+    static constexpr int SCALES = 2 * BN * 4;  // 2 slots x BN / 128 column blocks x 128 rows
+    static constexpr int SMEM = S * STAGE + STAGING + SCALES + (2 * S + 5) * 8 + 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
-constexpr int kWideThreads = 320;
-constexpr int W_TMA = 8, W_MMA = 9;
+constexpr int kWideThreads = 640;
+constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 18;
 
 // Tiles in groups of 16 rows of tiles, column by column within a group, so
 // that the CTAs at work share both operands' tiles in L2.
@@ -125,11 +133,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int by_tma, int *flags) {
     using W = Wide<BN>;
-    constexpr int S = W::S, COLS = BN / 2;
-    extern __shared__ uint8_t raw[];
-    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    constexpr int S = W::S, COLS = BN / 4;
+    extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *staging = base + S * W::STAGE;
-    uint64_t *bar0 = reinterpret_cast<uint64_t *>(staging + W::STAGING);
+    float *slots = reinterpret_cast<float *>(staging + W::STAGING);
+    uint64_t *bar0 = reinterpret_cast<uint64_t *>(slots + 2 * BN);
     const uint32_t bars = smem_u32(bar0);
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (S + s); };
@@ -147,8 +155,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(tfull(b), 1);
-            mbar_init(tempty(b), 8);
+            mbar_init(tfull(b), 1 + 64);  // the MMAs' commit and the scale warps' lanes
+            mbar_init(tempty(b), 16);
         }
         mbar_init(drained, 1);
         fence_mbar_init();
@@ -165,132 +173,166 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN, tiles = tiles_m * tiles_n;
     bool ok = true;
     int issued = 0;  // TMA: stages filled
-    if (warp == W_TMA) {
-        if (lane == 0) {
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == W_TMA) {
+            if (lane == 0) {
+                for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                    int tm, tn;
+                    tile_at(t, tiles_m, tiles_n, tm, tn);
+                    for (int b = 0; b < nkb; ++b, ++issued) {
+                        const int s = issued % S;
+                        if (!mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        const uint32_t at = smem_u32(base + s * W::STAGE);
+                        mbar_arrive_expect_tx(full(s), W::STAGE);
+                        tma_load_2d(at, &mapA, full(s), b * KB, tm * BM);
+                        tma_load_2d(at + kTile, &mapB, full(s), b * KB, tn * BN);
+                    }
+                }
+            }
+        } else if (warp == W_MMA) {
+            if (lane == 0) {
+                constexpr uint32_t idesc = idesc_e4m3(BM, BN);
+                int j = 0;
+                for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                    for (int b = 0; b < nkb; ++b, ++j) {
+                        const int s = j % S, buf = j & 1;
+                        if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        if (!mbar_wait(full(s), (j / S) & 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint64_t da = smem_desc_sw128(smem_u32(base + s * W::STAGE));
+                        const uint64_t db = smem_desc_sw128(smem_u32(base + s * W::STAGE + kTile));
+#pragma unroll
+                        for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, k > 0);
+                        mma_commit(empty(s));
+                        mma_commit(tfull(buf));
+                    }
+                }
+            }
+        } else {
+            // rows r and r + 64 of the tile; the next block's scales are loaded
+            // before this one's slot is waited for
+            const int r = (warp - W_SCALE) * 32 + lane;
+            constexpr int NB = BN / 128;
+            int j = 0;
             for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                 int tm, tn;
                 tile_at(t, tiles_m, tiles_n, tm, tn);
-                for (int b = 0; b < nkb; ++b, ++issued) {
-                    const int s = issued % S;
-                    if (!mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                    const uint32_t at = smem_u32(base + s * W::STAGE);
-                    mbar_arrive_expect_tx(full(s), W::STAGE);
-                    tma_load_2d(at, &mapA, full(s), b * KB, tm * BM);
-                    tma_load_2d(at + kTile, &mapB, full(s), b * KB, tn * BN);
-                }
-            }
-        }
-    } else if (warp == W_MMA) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(BM, BN);
-            int j = 0;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const float *a0 = sA + (int64_t)min(tm * BM + r, M - 1) * ldsA;
+                const float *a1 = sA + (int64_t)min(tm * BM + r + 64, M - 1) * ldsA;
+                const float *b0 = sB + (int64_t)(tn * NB) * ldsB;
+                // (a column block past N has no scales: its columns are not written)
+                const float *b1 = sB + (int64_t)min(tn * NB + NB - 1, (N - 1) / KB) * ldsB;
+                float x0 = __ldg(a0), x1 = __ldg(a1), y0 = __ldg(b0), y1 = __ldg(b1);
                 for (int b = 0; b < nkb; ++b, ++j) {
-                    const int s = j % S, buf = j & 1;
+                    const int buf = j & 1, nx = min(b + 1, nkb - 1);
+                    const float u0 = x0, u1 = x1, v0 = y0, v1 = y1;
+                    x0 = __ldg(a0 + nx);
+                    x1 = __ldg(a1 + nx);
+                    y0 = __ldg(b0 + nx);
+                    y1 = __ldg(b1 + nx);
                     if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                    if (!mbar_wait(full(s), (j / S) & 1, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint64_t da = smem_desc_sw128(smem_u32(base + s * W::STAGE));
-                    const uint64_t db = smem_desc_sw128(smem_u32(base + s * W::STAGE + kTile));
-#pragma unroll
-                    for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, k > 0);
-                    mma_commit(empty(s));
-                    mma_commit(tfull(buf));
+                    float *slot = slots + buf * BN;
+                    slot[r] = u0 * v0;
+                    slot[r + 64] = u1 * v0;
+                    if constexpr (NB == 2) {
+                        slot[128 + r] = u0 * v1;
+                        slot[128 + r + 64] = u1 * v1;
+                    }
+                    mbar_arrive(tfull(buf));
                 }
             }
         }
     } else {
-        const int q = warp & 3, half = warp >> 2;
-        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
-        uint8_t *stage = staging + warp * 4096;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        const int q = warp & 3, grp = warp >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + grp * COLS;
+        const float *my_scale = slots + grp * COLS / 128 * 128 + q * 32 + lane;
+        uint8_t *stage = staging + warp * 2048;
         int j = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            int tm, tn;
-            tile_at(t, tiles_m, tiles_n, tm, tn);
-            const int row = tm * BM + q * 32 + lane, col0 = tn * BN + half * COLS;
-            const bool valid = row < M;
-            const float *ra = sA + (int64_t)(valid ? row : 0) * ldsA;
-            // (a half past N has no scale row: its columns are not written)
-            const float *rb = sB + (int64_t)(col0 < N ? col0 / KB : 0) * ldsB;
             uint64_t acc[COLS / 2];
 #pragma unroll
             for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
-            float sa[4], sb[4], na[4], nb[4];
-            load_scales(na, ra, 0, nkb, valid);
-            load_scales(nb, rb, 0, nkb, true);
-            for (int b0 = 0; b0 < nkb && ok; b0 += 4) {
+            for (int b = 0; b < nkb; ++b, ++j) {
+                const int buf = j & 1;
+                // (one answer for the warp: its next steps are collective)
+                if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
+                tc_fence_after();
+                const float s = my_scale[buf * BN];
+                const uint64_t s2 = pack2(s, s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sa[i] = na[i], sb[i] = nb[i];
-                load_scales(na, ra, b0 + 4, nkb, valid);
-                load_scales(nb, rb, b0 + 4, nkb, true);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (b0 + i >= nkb) break;
-                    const int buf = j & 1;
-                    // (one answer for the warp: its next steps are collective)
-                    if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
-                    ++j;
-                    tc_fence_after();
-                    const float s = sa[i] * sb[i];
-                    const uint64_t s2 = pack2(s, s);
-#pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t r[32];
-                        tmem_ld_32x32b_x32(lanes + buf * BN + c * 32, r);
-                        tmem_ld_wait();
-                        if (c == COLS / 32 - 1) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(tempty(buf));
-                        }
-#pragma unroll
-                        for (int u = 0; u < 16; ++u) fma2(acc[c * 16 + u], pack2u(r[2 * u], r[2 * u + 1]), s2);
+                for (int c = 0; c < COLS / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(lanes + buf * BN + c * 32, r);
+                    tmem_ld_wait();
+                    if (c == COLS / 32 - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(tempty(buf));
                     }
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) fma2(acc[c * 16 + u], pack2u(r[2 * u], r[2 * u + 1]), s2);
                 }
             }
             if (!ok) break;
-            // 128 bytes of each of the warp's 32 rows at a time
-            constexpr int PIECE = 128 / (int)sizeof(T);
+            int tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            const int row0 = tm * BM + q * 32, col0 = tn * BN + grp * COLS;
+            if (bias) {
+#pragma unroll
+                for (int i = 0; i < COLS / 2; ++i) {
+                    float2 v = unpack2(acc[i]);
+                    v.x += __ldg(bias + min(col0 + 2 * i, N - 1));
+                    v.y += __ldg(bias + min(col0 + 2 * i + 1, N - 1));
+                    acc[i] = pack2(v.x, v.y);
+                }
+            }
+            if (epi != LONNX_EPI_NONE) {
+#pragma unroll
+                for (int i = 0; i < COLS / 2; ++i) {
+                    const float2 v = unpack2(acc[i]);
+                    acc[i] = epi == LONNX_EPI_RELU ? pack2(activate(v.x, LONNX_EPI_RELU), activate(v.y, LONNX_EPI_RELU))
+                                                   : pack2(lonnx_gelu_fast(v.x), lonnx_gelu_fast(v.y));
+                }
+            }
+            // 64 bytes of each of the warp's 32 rows at a time
+            constexpr int PIECE = 64 / (int)sizeof(T), CN = 16 / (int)sizeof(T);
 #pragma unroll
             for (int p = 0; p < COLS / PIECE; ++p) {
                 if (lane == 0) bulk_wait_group_read0();
                 __syncwarp();
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {  // 16-byte chunks of this lane's row
-                    constexpr int CN = 16 / (int)sizeof(T);
+                for (int c = 0; c < 4; ++c) {  // 16-byte chunks of this lane's row, 64B-swizzled
                     T out[CN];
 #pragma unroll
                     for (int u = 0; u < CN; u += 2) {
-                        const int e = p * PIECE + c * CN + u;
-                        float2 v = unpack2(acc[e / 2]);
-                        if (bias) {
-                            v.x += __ldg(bias + min(col0 + e, N - 1));
-                            v.y += __ldg(bias + min(col0 + e + 1, N - 1));
-                        }
-                        out[u] = from_f32<T>(activate(v.x, epi));
-                        out[u + 1] = from_f32<T>(activate(v.y, epi));
+                        const float2 v = unpack2(acc[(p * PIECE + c * CN + u) / 2]);
+                        out[u] = from_f32<T>(v.x);
+                        out[u + 1] = from_f32<T>(v.y);
                     }
-                    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
                         *reinterpret_cast<const uint4 *>(out);
                 }
                 const int col = col0 + p * PIECE;
                 if (by_tma) {
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && col < N && tm * BM + q * 32 < M) {
-                        tma_store_2d(&mapC, smem_u32(stage), col, tm * BM + q * 32);
+                    if (lane == 0 && col < N && row0 < M) {
+                        tma_store_2d(&mapC, smem_u32(stage), col, row0);
                         bulk_commit_group();
                     }
                 } else {
                     __syncwarp();
-                    const int rows = min(32, M - (tm * BM + q * 32));
-                    T *dst = C + (int64_t)(tm * BM + q * 32) * ldc + col;
-                    for (int r = 0; r < rows; ++r, dst += ldc)
-#pragma unroll
-                        for (int e = lane; e < PIECE; e += 32)
-                            if (col + e < N)
-                                dst[e] = *reinterpret_cast<const T *>(stage + r * 128 + ((((e * sizeof(T)) >> 4) ^ (r & 7)) << 4) +
-                                                                      ((e * sizeof(T)) & 15));
+                    // 32 elements of a row (16 of two rows) at a time
+                    constexpr int STEP = 32 / PIECE;
+                    const int e = lane % PIECE;
+                    const int rows = min(32, M - row0);
+                    T *dst = C + (int64_t)row0 * ldc + col + e;
+                    if (col + e < N)
+                        for (int r = lane / PIECE; r < rows; r += STEP)
+                            dst[(int64_t)r * ldc] = *reinterpret_cast<const T *>(
+                                stage + r * 64 + (((e / CN) ^ ((r >> 1) & 3)) << 4) + e % CN * sizeof(T));
                 }
             }
         }
@@ -536,17 +578,19 @@ __global__ void k_fp8_no_columns(const float *__restrict__ bias, T *__restrict__
 
 // ---- host side ------------------------------------------------------------------
 
-// row-major [rows, cols] of es-byte elements, leading dimension ld elements, box of 128 bytes x box_rows
+// row-major [rows, cols] of es-byte elements, leading dimension ld elements, box of
+// row_bytes (128 or 64, swizzled alike) x box_rows
 int tile_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int es, int64_t rows, int64_t cols,
-             int64_t ld, int box_rows) {
+             int64_t ld, int box_rows, int row_bytes = 128) {
     lonnx::tc::EncodeTiledFn enc = lonnx::tc::encode_tiled();
     if (!enc) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled unavailable");
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)(row_bytes / es), (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return LONNX_OK;
@@ -573,7 +617,7 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
         const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : p.dtype == LONNX_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        rc = tile_map(&mc, p.C, type, (int)sizeof(T), p.M, p.N, p.ldc, 32);
+        rc = tile_map(&mc, p.C, type, (int)sizeof(T), p.M, p.N, p.ldc, 32, 64);
         if (rc) return rc;
     }
     const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
