@@ -63,26 +63,6 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
     return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// two fp32 FMAs in one instruction: c += a * s
-__device__ __forceinline__ void fma2(uint64_t &c, uint64_t a, uint64_t s) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(s));
-}
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ uint64_t pack2u(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-
 // Four blocks' scales of one row, from block b (0 past the row's end)
 __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int b, int nkb, bool valid) {
 #pragma unroll
@@ -95,7 +75,7 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 //   warps 0-15   drain: each thread one row x BN / 4 columns in registers (four
 //                warps a scheduler: the TMEM loads of one hide behind the FMAs
 //                of the others); then the epilogue, 64 bytes of a row at a time
-//                through 2 KB of shared memory per warp and out by TMA (or,
+//                through twice 2 KB of shared memory per warp and out by TMA (or,
 //                where rows of C do not start on 16 bytes, by element stores
 //                that coalesce along rows)
 //   warp 16      TMA producer, warp 17 MMA issuer (and TMEM)
@@ -107,8 +87,8 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 template <int BN>
 struct Wide {
     static constexpr int STAGE = kTile + BN * KB;
-    static constexpr int S = BN == 256 ? 4 : 6;
-    static constexpr int STAGING = 16 * 2048;
+    static constexpr int S = BN == 256 ? 3 : 4;
+    static constexpr int STAGING = 16 * 4096;
     static constexpr int SCALES = 2 * BN * 4;  // 2 slots x BN / 128 column blocks x 128 rows
     static constexpr int SMEM = S * STAGE + STAGING + SCALES + (2 * S + 5) * 8 + 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
@@ -162,13 +142,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         fence_mbar_init();
     }
     if (warp == W_MMA) {
-        tmem_alloc(smem_u32(tmem_slot), 2 * BN);
+        tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    // all 512 columns, which start at 0: a constant for the MMA's uniform registers
+    constexpr uint32_t tmem = 0;
 
     const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN, tiles = tiles_m * tiles_n;
     bool ok = true;
@@ -191,22 +172,26 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 }
             }
         } else if (warp == W_MMA) {
-            if (lane == 0) {
-                constexpr uint32_t idesc = idesc_e4m3(BM, BN);
-                int j = 0;
-                for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                    for (int b = 0; b < nkb; ++b, ++j) {
-                        const int s = j % S, buf = j & 1;
-                        if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                        if (!mbar_wait(full(s), (j / S) & 1, abort_flag)) { ok = false; break; }
-                        tc_fence_after();
-                        const uint64_t da = smem_desc_sw128(smem_u32(base + s * W::STAGE));
-                        const uint64_t db = smem_desc_sw128(smem_u32(base + s * W::STAGE + kTile));
+            // the whole warp walks the loop and one elected lane issues, so that
+            // descriptors stay in uniform registers
+            constexpr uint32_t idesc = idesc_e4m3(BM, BN);
+            const uint64_t desc0 = smem_desc_sw128(smem_u32(base));
+            int j = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                for (int b = 0; b < nkb; ++b, ++j) {
+                    const int s = j % S, buf = j & 1;
+                    const bool ready = mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag) &&
+                                       mbar_wait(full(s), (j / S) & 1, abort_flag);
+                    if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t da = desc0 + (uint32_t)(s * (W::STAGE / 16)), db = da + kTile / 16;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, k > 0);
                         mma_commit(empty(s));
                         mma_commit(tfull(buf));
                     }
+                    __syncwarp();
                 }
             }
         } else {
@@ -248,19 +233,17 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const int q = warp & 3, grp = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + grp * COLS;
         const float *my_scale = slots + grp * COLS / 128 * 128 + q * 32 + lane;
-        uint8_t *stage = staging + warp * 2048;
         int j = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            uint64_t acc[COLS / 2];
+            float acc[COLS];
 #pragma unroll
-            for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
             for (int b = 0; b < nkb; ++b, ++j) {
                 const int buf = j & 1;
                 // (one answer for the warp: its next steps are collective)
                 if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
                 tc_fence_after();
                 const float s = my_scale[buf * BN];
-                const uint64_t s2 = pack2(s, s);
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
                     uint32_t r[32];
@@ -272,45 +255,37 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         if (lane == 0) mbar_arrive(tempty(buf));
                     }
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) fma2(acc[c * 16 + u], pack2u(r[2 * u], r[2 * u + 1]), s2);
+                    for (int u = 0; u < 32; ++u) acc[c * 32 + u] = fmaf(__uint_as_float(r[u]), s, acc[c * 32 + u]);
                 }
             }
             if (!ok) break;
             int tm, tn;
             tile_at(t, tiles_m, tiles_n, tm, tn);
             const int row0 = tm * BM + q * 32, col0 = tn * BN + grp * COLS;
-            if (bias) {
-#pragma unroll
-                for (int i = 0; i < COLS / 2; ++i) {
-                    float2 v = unpack2(acc[i]);
-                    v.x += __ldg(bias + min(col0 + 2 * i, N - 1));
-                    v.y += __ldg(bias + min(col0 + 2 * i + 1, N - 1));
-                    acc[i] = pack2(v.x, v.y);
-                }
-            }
-            if (epi != LONNX_EPI_NONE) {
-#pragma unroll
-                for (int i = 0; i < COLS / 2; ++i) {
-                    const float2 v = unpack2(acc[i]);
-                    acc[i] = epi == LONNX_EPI_RELU ? pack2(activate(v.x, LONNX_EPI_RELU), activate(v.y, LONNX_EPI_RELU))
-                                                   : pack2(lonnx_gelu_fast(v.x), lonnx_gelu_fast(v.y));
-                }
-            }
-            // 64 bytes of each of the warp's 32 rows at a time
+            // 64 bytes of each of the warp's 32 rows at a time, through two buffers:
+            // the activation of one piece runs while the last one leaves
             constexpr int PIECE = 64 / (int)sizeof(T), CN = 16 / (int)sizeof(T);
 #pragma unroll
             for (int p = 0; p < COLS / PIECE; ++p) {
-                if (lane == 0) bulk_wait_group_read0();
+                uint8_t *stage = staging + warp * 4096 + (p & 1) * 2048;
+                if (bias) {
+#pragma unroll
+                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] += __ldg(bias + min(col0 + i, N - 1));
+                }
+                if (epi == LONNX_EPI_RELU) {
+#pragma unroll
+                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] = activate(acc[i], LONNX_EPI_RELU);
+                } else if (epi == LONNX_EPI_GELU_ERF) {
+#pragma unroll
+                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] = lonnx_gelu_fast(acc[i]);
+                }
+                if (lane == 0) bulk_wait_group_read1();
                 __syncwarp();
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {  // 16-byte chunks of this lane's row, 64B-swizzled
                     T out[CN];
 #pragma unroll
-                    for (int u = 0; u < CN; u += 2) {
-                        const float2 v = unpack2(acc[(p * PIECE + c * CN + u) / 2]);
-                        out[u] = from_f32<T>(v.x);
-                        out[u + 1] = from_f32<T>(v.y);
-                    }
+                    for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[p * PIECE + c * CN + u]);
                     *reinterpret_cast<uint4 *>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
                         *reinterpret_cast<const uint4 *>(out);
                 }
@@ -318,9 +293,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 if (by_tma) {
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && col < N && row0 < M) {
-                        tma_store_2d(&mapC, smem_u32(stage), col, row0);
-                        bulk_commit_group();
+                    if (lane == 0) {
+                        if (col < N && row0 < M) tma_store_2d(&mapC, smem_u32(stage), col, row0);
+                        bulk_commit_group();  // (an empty group keeps the count)
                     }
                 } else {
                     __syncwarp();
@@ -345,8 +320,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     __syncthreads();
     if (*abort_flag) {
         // copies and MMAs in flight end before shared memory and TMEM go (bounded waits)
-        if (warp == W_MMA && lane == 0) {
-            mma_commit(drained);
+        if (warp == W_MMA) {
+            if (elect_one()) mma_commit(drained);  // the lane that issued
             mbar_wait(drained, 0, nullptr, 400000000ll);
         }
         if (warp == W_TMA && lane == 0)
@@ -356,7 +331,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     __syncthreads();
     if (warp == W_MMA) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -465,9 +440,9 @@ __global__ void __launch_bounds__(kSplitThreads)
         constexpr int PER = (TOK + 31) / 32;  // rows of A whose scales a lane fetches
         float *my = scales + warp * 4 * TOK;  // [4 blocks][TOK], this warp's copy
         const float *rb = sB + (int64_t)(n0 / KB) * ldsB;
-        uint64_t acc[TOK / 2];
+        float acc[TOK];
 #pragma unroll
-        for (int i = 0; i < TOK / 2; ++i) acc[i] = 0;
+        for (int i = 0; i < TOK; ++i) acc[i] = 0.0f;
         float na[PER][4], nb[4];
         auto fetch = [&](int b) {
 #pragma unroll
@@ -505,12 +480,15 @@ __global__ void __launch_bounds__(kSplitThreads)
                         __syncwarp();
                         if (lane == 0) mbar_arrive(tempty(buf));
                     }
-                    const ulonglong2 *s4 = reinterpret_cast<const ulonglong2 *>(my + i * TOK + c * CH);
+                    const float4 *s4 = reinterpret_cast<const float4 *>(my + i * TOK + c * CH);
 #pragma unroll
                     for (int u = 0; u < CH / 4; ++u) {
-                        const ulonglong2 s = s4[u];
-                        fma2(acc[c * (CH / 2) + 2 * u], pack2u(r[4 * u], r[4 * u + 1]), s.x);
-                        fma2(acc[c * (CH / 2) + 2 * u + 1], pack2u(r[4 * u + 2], r[4 * u + 3]), s.y);
+                        const float4 s = s4[u];
+                        float *a = acc + c * CH + 4 * u;
+                        a[0] = fmaf(__uint_as_float(r[4 * u]), s.x, a[0]);
+                        a[1] = fmaf(__uint_as_float(r[4 * u + 1]), s.y, a[1]);
+                        a[2] = fmaf(__uint_as_float(r[4 * u + 2]), s.z, a[2]);
+                        a[3] = fmaf(__uint_as_float(r[4 * u + 3]), s.w, a[3]);
                     }
                 }
             }
@@ -518,11 +496,7 @@ __global__ void __launch_bounds__(kSplitThreads)
         // the last block's MMAs have read the stages: the sums may go over them
         if (ok) {
 #pragma unroll
-            for (int i = 0; i < TOK / 2; ++i) {
-                const float2 v = unpack2(acc[i]);
-                sums[(2 * i) * BM + threadIdx.x] = v.x;
-                sums[(2 * i + 1) * BM + threadIdx.x] = v.y;
-            }
+            for (int i = 0; i < TOK; ++i) sums[i * BM + threadIdx.x] = acc[i];
         }
     }
     if (!ok) {
