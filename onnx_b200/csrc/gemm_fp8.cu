@@ -72,29 +72,37 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 // ---- wide tiles -----------------------------------------------------------------
 //
 // CTA = 20 warps, one per SM, walking tiles of 128 x BN:
-//   warps 0-15   drain: each thread one row x BN / 4 columns in registers (four
+//   warps 0-15   drain: each thread one row x 64 columns in registers (four
 //                warps a scheduler: the TMEM loads of one hide behind the FMAs
 //                of the others); then the epilogue, 64 bytes of a row at a time
-//                through twice 2 KB of shared memory per warp and out by TMA (or,
-//                where rows of C do not start on 16 bytes, by element stores
-//                that coalesce along rows)
-//   warp 16      TMA producer, warp 17 MMA issuer (and TMEM)
-//   warps 18, 19 the block's scales: sA[m, b] * sB[n / 128, b] of the tile's 128
+//                through twice 2 KB of shared memory per warp and out by TMA
+//                (or, where rows of C do not start on 16 bytes, by element
+//                stores that coalesce along rows)
+//   warp 16      TMA producer
+//   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM): waits and
+//                loop around a block's four MMAs took a single issuer 350 of
+//                860 cycles
+//   warp 19      the block's scales: sA[m, b] * sB[n / 128, b] of the tile's 128
 //                rows and BN / 128 column blocks into shared memory, one slot
 //                per TMEM buffer, under the same barriers
+// BN = 256 has one set of 16 drain warps and two TMEM buffers.  BN = 128 has two
+// sets of 8, with two buffers each, that take turns at tiles: the epilogue of
+// one set runs beside the other's blocks.
 // The drain warps take registers from the other four (setmaxnreg): 512 x 112 +
 // 128 x 32 = 640 x 96, the launch's.
 template <int BN>
 struct Wide {
     static constexpr int STAGE = kTile + BN * KB;
-    static constexpr int S = BN == 256 ? 3 : 4;
+    static constexpr int S = BN == 256 ? 3 : 5;
+    static constexpr int SETS = 256 / BN, BUFS = 2 * SETS;
     static constexpr int STAGING = 16 * 4096;
-    static constexpr int SCALES = 2 * BN * 4;  // 2 slots x BN / 128 column blocks x 128 rows
-    static constexpr int SMEM = S * STAGE + STAGING + SCALES + (2 * S + 5) * 8 + 8;
+    static constexpr int SCALES = BUFS * BN * 4;  // a slot per buffer: BN / 128 column blocks x 128 rows
+    static constexpr int BARS = 2 * S + 2 * BUFS + 1;
+    static constexpr int SMEM = S * STAGE + STAGING + SCALES + BARS * 8 + 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 constexpr int kWideThreads = 640;
-constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 18;
+constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 19;
 
 // Tiles in groups of 16 rows of tiles, column by column within a group, so
 // that the CTAs at work share both operands' tiles in L2.
@@ -113,19 +121,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int by_tma, int *flags) {
     using W = Wide<BN>;
-    constexpr int S = W::S, COLS = BN / 4;
+    constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *staging = base + S * W::STAGE;
     float *slots = reinterpret_cast<float *>(staging + W::STAGING);
-    uint64_t *bar0 = reinterpret_cast<uint64_t *>(slots + 2 * BN);
+    uint64_t *bar0 = reinterpret_cast<uint64_t *>(slots + W::BUFS * BN);
     const uint32_t bars = smem_u32(bar0);
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (S + s); };
     auto tfull = [&](int b) { return bars + 8 * (2 * S + b); };
-    auto tempty = [&](int b) { return bars + 8 * (2 * S + 2 + b); };
-    const uint32_t drained = bars + 8 * (2 * S + 4);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + 2 * S + 5);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + 2 * S + 5) + 1;
+    auto tempty = [&](int b) { return bars + 8 * (2 * S + W::BUFS + b); };
+    const uint32_t drained = bars + 8 * (2 * S + 2 * W::BUFS);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + W::BARS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + W::BARS) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -134,11 +142,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(tfull(b), 1 + 64);  // the MMAs' commit and the scale warps' lanes
-            mbar_init(tempty(b), 16);
+        for (int b = 0; b < W::BUFS; ++b) {
+            mbar_init(tfull(b), 1 + 32);  // the MMAs' commit and the scale warp's lanes
+            mbar_init(tempty(b), 16 / SETS);
         }
-        mbar_init(drained, 1);
+        mbar_init(drained, 2);
         fence_mbar_init();
     }
     if (warp == W_MMA) {
@@ -171,17 +179,26 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     }
                 }
             }
-        } else if (warp == W_MMA) {
+        } else if (warp < W_SCALE) {
             // the whole warp walks the loop and one elected lane issues, so that
             // descriptors stay in uniform registers
             constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             const uint64_t desc0 = smem_desc_sw128(smem_u32(base));
-            int j = 0;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                for (int b = 0; b < nkb; ++b, ++j) {
-                    const int s = j % S, buf = j & 1;
-                    const bool ready = mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag) &&
-                                       mbar_wait(full(s), (j / S) & 1, abort_flag);
+            // Issuer e takes blocks e, e + 2, .. of the ring's order.  A parity wait
+            // must not be two phases ahead of its barrier: the ring's order holds
+            // the issuers within S blocks of each other, and full() is waited for
+            // before tempty(), which then is at most one phase ahead: the block two
+            // before in its buffer is this issuer's own, or at least S before.
+            int js[2] = {0, 0}, i = 0;  // blocks of each set, blocks of all
+            for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
+                const int set = SETS == 2 ? n & 1 : 0;
+                int j = js[set];
+                js[set] += nkb;
+                for (int b = 0; b < nkb; ++b, ++j, ++i) {
+                    if ((i & 1) != warp - W_MMA) continue;
+                    const int s = i % S, buf = 2 * set + (j & 1);
+                    const bool ready = mbar_wait(full(s), (i / S) & 1, abort_flag) &&
+                                       mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag);
                     if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                     tc_fence_after();
                     const uint64_t da = desc0 + (uint32_t)(s * (W::STAGE / 16)), db = da + kTile / 16;
@@ -195,53 +212,61 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 }
             }
         } else {
-            // rows r and r + 64 of the tile; the next block's scales are loaded
+            // rows lane + 32 i of the tile; the next block's scales are loaded
             // before this one's slot is waited for
-            const int r = (warp - W_SCALE) * 32 + lane;
             constexpr int NB = BN / 128;
-            int j = 0;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            int js[2] = {0, 0};  // blocks of each set
+            for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
+                const int set = SETS == 2 ? n & 1 : 0;
                 int tm, tn;
                 tile_at(t, tiles_m, tiles_n, tm, tn);
-                const float *a0 = sA + (int64_t)min(tm * BM + r, M - 1) * ldsA;
-                const float *a1 = sA + (int64_t)min(tm * BM + r + 64, M - 1) * ldsA;
-                const float *b0 = sB + (int64_t)(tn * NB) * ldsB;
-                // (a column block past N has no scales: its columns are not written)
-                const float *b1 = sB + (int64_t)min(tn * NB + NB - 1, (N - 1) / KB) * ldsB;
-                float x0 = __ldg(a0), x1 = __ldg(a1), y0 = __ldg(b0), y1 = __ldg(b1);
+                const float *ra[4], *rb[NB];
+                float x[4], y[NB];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ra[i] = sA + (int64_t)min(tm * BM + lane + 32 * i, M - 1) * ldsA;
+                    x[i] = __ldg(ra[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    // (a column block past N has no scales: its columns are not written)
+                    rb[i] = sB + (int64_t)min(tn * NB + i, (N - 1) / KB) * ldsB;
+                    y[i] = __ldg(rb[i]);
+                }
+                int j = js[set];
+                js[set] += nkb;
                 for (int b = 0; b < nkb; ++b, ++j) {
-                    const int buf = j & 1, nx = min(b + 1, nkb - 1);
-                    const float u0 = x0, u1 = x1, v0 = y0, v1 = y1;
-                    x0 = __ldg(a0 + nx);
-                    x1 = __ldg(a1 + nx);
-                    y0 = __ldg(b0 + nx);
-                    y1 = __ldg(b1 + nx);
+                    const int buf = 2 * set + (j & 1), nx = min(b + 1, nkb - 1);
                     if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
                     float *slot = slots + buf * BN;
-                    slot[r] = u0 * v0;
-                    slot[r + 64] = u1 * v0;
-                    if constexpr (NB == 2) {
-                        slot[128 + r] = u0 * v1;
-                        slot[128 + r + 64] = u1 * v1;
-                    }
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) slot[n * 128 + lane + 32 * i] = x[i] * y[n];
                     mbar_arrive(tfull(buf));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = __ldg(ra[i] + nx);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) y[i] = __ldg(rb[i] + nx);
                 }
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         const int q = warp & 3, grp = warp >> 2;
-        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + grp * COLS;
-        const float *my_scale = slots + grp * COLS / 128 * 128 + q * 32 + lane;
-        int j = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int set = SETS == 2 ? grp >> 1 : 0, part = SETS == 2 ? grp & 1 : grp;  // 64 columns of the set's tile
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + 2 * set * BN + part * COLS;
+        const bool bias4 = ((uintptr_t)bias & 15) == 0;
+        const float *my_scale = slots + 2 * set * BN + part / 2 * 128 + q * 32 + lane;
+        int j = 0;  // blocks of the set
+        for (int t = blockIdx.x + set * gridDim.x; t < tiles && ok; t += SETS * gridDim.x) {
             float acc[COLS];
 #pragma unroll
             for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
             for (int b = 0; b < nkb; ++b, ++j) {
                 const int buf = j & 1;
                 // (one answer for the warp: its next steps are collective)
-                if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, mbar_wait(tfull(2 * set + buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
                 tc_fence_after();
                 const float s = my_scale[buf * BN];
 #pragma unroll
@@ -252,7 +277,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     if (c == COLS / 32 - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(tempty(buf));
+                        if (lane == 0) mbar_arrive(tempty(2 * set + buf));
                     }
 #pragma unroll
                     for (int u = 0; u < 32; ++u) acc[c * 32 + u] = fmaf(__uint_as_float(r[u]), s, acc[c * 32 + u]);
@@ -261,7 +286,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (!ok) break;
             int tm, tn;
             tile_at(t, tiles_m, tiles_n, tm, tn);
-            const int row0 = tm * BM + q * 32, col0 = tn * BN + grp * COLS;
+            const int row0 = tm * BM + q * 32, col0 = tn * BN + part * COLS;
             // 64 bytes of each of the warp's 32 rows at a time, through two buffers:
             // the activation of one piece runs while the last one leaves
             constexpr int PIECE = 64 / (int)sizeof(T), CN = 16 / (int)sizeof(T);
@@ -269,8 +294,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             for (int p = 0; p < COLS / PIECE; ++p) {
                 uint8_t *stage = staging + warp * 4096 + (p & 1) * 2048;
                 if (bias) {
+                    if (bias4 && col0 + COLS <= N) {
 #pragma unroll
-                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] += __ldg(bias + min(col0 + i, N - 1));
+                        for (int i = p * PIECE; i < (p + 1) * PIECE; i += 4) {
+                            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + col0 + i));
+                            acc[i] += v.x;
+                            acc[i + 1] += v.y;
+                            acc[i + 2] += v.z;
+                            acc[i + 3] += v.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] += __ldg(bias + min(col0 + i, N - 1));
+                    }
                 }
                 if (epi == LONNX_EPI_RELU) {
 #pragma unroll
@@ -320,7 +356,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     __syncthreads();
     if (*abort_flag) {
         // copies and MMAs in flight end before shared memory and TMEM go (bounded waits)
-        if (warp == W_MMA) {
+        if (warp == W_MMA || warp == W_MMA + 1) {
             if (elect_one()) mma_commit(drained);  // the lane that issued
             mbar_wait(drained, 0, nullptr, 400000000ll);
         }
