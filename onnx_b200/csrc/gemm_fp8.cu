@@ -287,63 +287,84 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             int tm, tn;
             tile_at(t, tiles_m, tiles_n, tm, tn);
             const int row0 = tm * BM + q * 32, col0 = tn * BN + part * COLS;
-            // 64 bytes of each of the warp's 32 rows at a time, through two buffers:
-            // the activation of one piece runs while the last one leaves
-            constexpr int PIECE = 64 / (int)sizeof(T), CN = 16 / (int)sizeof(T);
-#pragma unroll
-            for (int p = 0; p < COLS / PIECE; ++p) {
-                uint8_t *stage = staging + warp * 4096 + (p & 1) * 2048;
+            auto finish = [&](int i) {  // 16 bytes of C from column i
+                constexpr int CN = 16 / (int)sizeof(T);
                 if (bias) {
                     if (bias4 && col0 + COLS <= N) {
 #pragma unroll
-                        for (int i = p * PIECE; i < (p + 1) * PIECE; i += 4) {
-                            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + col0 + i));
-                            acc[i] += v.x;
-                            acc[i + 1] += v.y;
-                            acc[i + 2] += v.z;
-                            acc[i + 3] += v.w;
+                        for (int u = 0; u < CN; u += 4) {
+                            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + col0 + i + u));
+                            acc[i + u] += v.x;
+                            acc[i + u + 1] += v.y;
+                            acc[i + u + 2] += v.z;
+                            acc[i + u + 3] += v.w;
                         }
                     } else {
 #pragma unroll
-                        for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] += __ldg(bias + min(col0 + i, N - 1));
+                        for (int u = 0; u < CN; ++u) acc[i + u] += __ldg(bias + min(col0 + i + u, N - 1));
                     }
                 }
                 if (epi == LONNX_EPI_RELU) {
 #pragma unroll
-                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] = activate(acc[i], LONNX_EPI_RELU);
+                    for (int u = 0; u < CN; ++u) acc[i + u] = activate(acc[i + u], LONNX_EPI_RELU);
                 } else if (epi == LONNX_EPI_GELU_ERF) {
 #pragma unroll
-                    for (int i = p * PIECE; i < (p + 1) * PIECE; ++i) acc[i] = lonnx_gelu_fast(acc[i]);
+                    for (int u = 0; u < CN; ++u) acc[i + u] = lonnx_gelu_fast(acc[i + u]);
                 }
-                if (lane == 0) bulk_wait_group_read1();
-                __syncwarp();
+                T out[CN];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {  // 16-byte chunks of this lane's row, 64B-swizzled
-                    T out[CN];
+                for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[i + u]);
+                return *reinterpret_cast<const uint4 *>(out);
+            };
+            constexpr int CN = 16 / (int)sizeof(T);
+            uint8_t *stage = staging + warp * 4096;
+            if (by_tma) {
+                // 64 bytes of each of the warp's 32 rows at a time, through two
+                // buffers: one piece is computed while the last one leaves
+                constexpr int PIECE = 64 / (int)sizeof(T);
 #pragma unroll
-                    for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[p * PIECE + c * CN + u]);
-                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-                        *reinterpret_cast<const uint4 *>(out);
-                }
-                const int col = col0 + p * PIECE;
-                if (by_tma) {
+                for (int p = 0; p < COLS / PIECE; ++p) {
+                    uint8_t *buf = stage + (p & 1) * 2048;
+                    if (lane == 0) bulk_wait_group_read1();
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)  // 16-byte chunks of this lane's row, 64B-swizzled
+                        *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = finish(p * PIECE + c * CN);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        if (col < N && row0 < M) tma_store_2d(&mapC, smem_u32(stage), col, row0);
+                        const int col = col0 + p * PIECE;
+                        if (col < N && row0 < M) tma_store_2d(&mapC, smem_u32(buf), col, row0);
                         bulk_commit_group();  // (an empty group keeps the count)
                     }
-                } else {
+                }
+            } else {
+                // 128 bytes of a row at a time by element stores, the warp along
+                // the row; 8 rows' loads and stores in flight
+                constexpr int PIECE = 128 / (int)sizeof(T);
+#pragma unroll
+                for (int p = 0; p < COLS / PIECE; ++p) {
                     __syncwarp();
-                    // 32 elements of a row (16 of two rows) at a time
-                    constexpr int STEP = 32 / PIECE;
-                    const int e = lane % PIECE;
-                    const int rows = min(32, M - row0);
-                    T *dst = C + (int64_t)row0 * ldc + col + e;
-                    if (col + e < N)
-                        for (int r = lane / PIECE; r < rows; r += STEP)
-                            dst[(int64_t)r * ldc] = *reinterpret_cast<const T *>(
-                                stage + r * 64 + (((e / CN) ^ ((r >> 1) & 3)) << 4) + e % CN * sizeof(T));
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = finish(p * PIECE + c * CN);
+                    __syncwarp();
+                    const int rows = M - row0;
+#pragma unroll
+                    for (int e0 = 0; e0 < PIECE; e0 += 32) {
+                        const int e = e0 + lane, col = col0 + p * PIECE + e;
+                        T *dst = C + (int64_t)row0 * ldc + col;
+#pragma unroll
+                        for (int r0 = 0; r0 < 32; r0 += 8) {
+                            T x[8];
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                x[r] = *reinterpret_cast<const T *>(stage + (r0 + r) * 128 + (((e / CN) ^ r) << 4) + e % CN * sizeof(T));
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                if (col < N && r0 + r < rows) dst[(int64_t)(r0 + r) * ldc] = x[r];
+                        }
+                    }
                 }
             }
         }
@@ -373,36 +394,46 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 
 // ---- few rows: K split over a cluster ---------------------------------------------
 //
-// One tile of 128 rows of B (the tensor core's rows) x TOK rows of A (its
-// columns) per cluster; each CTA of the cluster takes a run of K's blocks.
+// Tiles of 128 rows of B (the tensor core's rows) x TOK rows of A (its columns),
+// each by a cluster of CTAs that take a run of K's blocks each; where one CTA
+// takes all of K (parts = 1), it walks several tiles, the next one's loads
+// running under the epilogue.
 //   warps 0-3  drain: each thread one row of B x TOK sums in registers
 //   warp 4     TMA producer, warp 5 MMA issuer (and TMEM)
-// The CTAs' sums meet in shared memory, TOK / CTAs rows of A to each CTA, added
-// in the CTAs' order.  A thread writes consecutive elements of C's rows with
-// its neighbours, so C needs no alignment.
+// A thread writes consecutive elements of C's rows with its neighbours, so C
+// needs no alignment.  The CTAs' sums meet in shared memory, TOK / parts rows of
+// A to each CTA, added in the CTAs' order.
 constexpr int kSplitThreads = 192;
 template <int TOK>
 struct Split {
     static constexpr int STAGE = kTile + TOK * KB;
     static constexpr int TMEM = 2 * TOK < 32 ? 32 : 2 * TOK;
     static constexpr int SCALES = 4 * 4 * TOK * 4;  // 4 warps x 4 blocks
-    static constexpr int MAX_STAGES = 8 * 18432 / STAGE;
-    static int smem(int stages) {
-        return 1024 + std::max(stages * STAGE, TOK * BM * 4) + SCALES + (2 * MAX_STAGES + 5) * 8 + 8;
+    static constexpr int MAX_STAGES = TOK == 16 ? 4 : 3;
+    static constexpr int BARS = 2 * MAX_STAGES + 5;
+    static constexpr int PER_SM = TOK == 128 ? 2 : 3;  // by shared memory
+    static int smem(int stages, int parts) {
+        return std::max(stages * STAGE, parts > 1 ? TOK * BM * 4 : 0) + SCALES + BARS * 8 + 8;
     }
 };
 
-template <int TOK>
-__global__ void __launch_bounds__(kSplitThreads)
+template <typename T>
+__device__ __forceinline__ void finish_store(T *C, int64_t at, float v, float bias, int epi) {
+    C[at] = from_f32<T>(activate(v + bias, epi));
+}
+
+template <int TOK, typename T>
+__global__ void __launch_bounds__(kSplitThreads, TOK == 128 ? 1 : TOK == 64 ? 2 : 3)
     k_fp8_split(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                 const float *__restrict__ sA, int64_t ldsA, const float *__restrict__ sB, int64_t ldsB,
-                const float *__restrict__ bias, void *__restrict__ C, int dtype, int64_t ldc, int M, int N, int nkb,
-                int stages, int epi, int *flags) {
+                const float *__restrict__ bias, T *__restrict__ C, int64_t ldc, int M, int N, int nkb, int stages,
+                int epi, int *flags) {
     using P = Split<TOK>;
-    extern __shared__ uint8_t raw[];
-    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    float *sums = reinterpret_cast<float *>(base);  // [TOK][128], over the stages once they are read
-    float *scales = reinterpret_cast<float *>(base + max(stages * P::STAGE, TOK * BM * 4));
+    extern __shared__ __align__(1024) uint8_t base[];
+    auto cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    float *sums = reinterpret_cast<float *>(base);  // parts > 1: [TOK][128], over the stages once they are read
+    float *scales = reinterpret_cast<float *>(base + max(stages * P::STAGE, parts > 1 ? TOK * BM * 4 : 0));
     uint64_t *bar0 = reinterpret_cast<uint64_t *>(scales + 16 * TOK);
     const uint32_t bars = smem_u32(bar0);
     auto full = [&](int s) { return bars + 8 * s; };
@@ -410,13 +441,12 @@ __global__ void __launch_bounds__(kSplitThreads)
     auto tfull = [&](int b) { return bars + 8 * (2 * P::MAX_STAGES + b); };
     auto tempty = [&](int b) { return bars + 8 * (2 * P::MAX_STAGES + 2 + b); };
     const uint32_t drained = bars + 8 * (2 * P::MAX_STAGES + 4);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + 2 * P::MAX_STAGES + 5);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + 2 * P::MAX_STAGES + 5) + 1;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + P::BARS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + P::BARS) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto cluster = cg::this_cluster();
-    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-    const int tiles_n = (N + BM - 1) / BM;
-    const int tile = blockIdx.x / parts, tm = tile / tiles_n, n0 = (tile - tm * tiles_n) * BM, m0 = tm * TOK;
+    const int tiles_n = (N + BM - 1) / BM, tiles_m = (M + TOK - 1) / TOK, tiles = tiles_n * tiles_m;
+    // (parts > 1: the grid has a cluster for each tile)
+    const int first_tile = blockIdx.x / parts, tile_step = gridDim.x / parts;
     const int b_first = (int)((int64_t)nkb * part / parts), b_last = (int)((int64_t)nkb * (part + 1) / parts);
     const int blocks = b_last - b_first;
 
@@ -446,93 +476,117 @@ __global__ void __launch_bounds__(kSplitThreads)
     int issued = 0;
     if (warp == 4) {
         if (lane == 0) {
-            for (; issued < blocks; ++issued) {
-                const int s = issued % stages;
-                if (!mbar_wait(empty(s), ((issued / stages) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                const uint32_t at = smem_u32(base + s * P::STAGE);
-                mbar_arrive_expect_tx(full(s), P::STAGE);
-                tma_load_2d(at, &mapB, full(s), (b_first + issued) * KB, n0);
-                tma_load_2d(at + kTile, &mapA, full(s), (b_first + issued) * KB, m0);
+            for (int tile = first_tile, s = 0, phase = 1; tile < tiles && ok; tile += tile_step) {
+                const int tm = tile / tiles_n, n0 = (tile - tm * tiles_n) * BM;
+                for (int b = b_first; b < b_last; ++b, ++issued) {
+                    if (!mbar_wait(empty(s), phase, abort_flag)) { ok = false; break; }
+                    const uint32_t at = smem_u32(base + s * P::STAGE);
+                    mbar_arrive_expect_tx(full(s), P::STAGE);
+                    tma_load_2d(at, &mapB, full(s), b * KB, n0);
+                    tma_load_2d(at + kTile, &mapA, full(s), b * KB, tm * TOK);
+                    if (++s == stages) s = 0, phase ^= 1;
+                }
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(BM, TOK);
-            for (int j = 0; j < blocks; ++j) {
-                const int s = j % stages, buf = j & 1;
-                if (!mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                if (!mbar_wait(full(s), (j / stages) & 1, abort_flag)) { ok = false; break; }
+        constexpr uint32_t idesc = idesc_e4m3(BM, TOK);
+        const uint64_t desc0 = smem_desc_sw128(smem_u32(base));
+        const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+        int j = 0;
+        for (int tile = first_tile, s = 0, phase = 0; tile < tiles && ok; tile += tile_step) {
+            for (int b = 0; b < blocks; ++b, ++j) {
+                const int buf = j & 1;
+                const bool ready = mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag) &&
+                                   mbar_wait(full(s), phase, abort_flag);
+                if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                 tc_fence_after();
-                const uint64_t da = smem_desc_sw128(smem_u32(base + s * P::STAGE));
-                const uint64_t db = smem_desc_sw128(smem_u32(base + s * P::STAGE + kTile));
+                const uint64_t da = desc0 + (uint32_t)(s * (P::STAGE / 16)), db = da + kTile / 16;
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < KB / 32; ++k) mma_fp8(tmem + buf * TOK, da + 2 * k, db + 2 * k, idesc, k > 0);
-                mma_commit(empty(s));
-                mma_commit(tfull(buf));
+                    for (int k = 0; k < KB / 32; ++k) mma_fp8(d0 + buf * TOK, da + 2 * k, db + 2 * k, idesc, k > 0);
+                    mma_commit(empty(s));
+                    mma_commit(tfull(buf));
+                }
+                __syncwarp();
+                if (++s == stages) s = 0, phase ^= 1;
             }
         }
     } else {
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
         constexpr int PER = (TOK + 31) / 32;  // rows of A whose scales a lane fetches
         float *my = scales + warp * 4 * TOK;  // [4 blocks][TOK], this warp's copy
-        const float *rb = sB + (int64_t)(n0 / KB) * ldsB;
-        float acc[TOK];
+        int j = 0;
+        for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
+            const int tm = tile / tiles_n, n0 = (tile - tm * tiles_n) * BM, m0 = tm * TOK;
+            const float *rb = sB + (int64_t)(n0 / KB) * ldsB;
+            float acc[TOK];
 #pragma unroll
-        for (int i = 0; i < TOK; ++i) acc[i] = 0.0f;
-        float na[PER][4], nb[4];
-        auto fetch = [&](int b) {
+            for (int i = 0; i < TOK; ++i) acc[i] = 0.0f;
+            float na[PER][4], nb[4];
+            auto fetch = [&](int b) {
 #pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                const int m = m0 + lane + 32 * p;
-                const bool valid = m < M && lane + 32 * p < TOK;
-                load_scales(na[p], sA + (int64_t)(valid ? m : 0) * ldsA, b, b_last, valid);
-            }
-            load_scales(nb, rb, b, b_last, true);
-        };
-        fetch(b_first);
-        for (int b0 = 0; b0 < blocks && ok; b0 += 4) {
-            __syncwarp();
+                for (int p = 0; p < PER; ++p) {
+                    const int m = m0 + lane + 32 * p;
+                    const bool valid = m < M && lane + 32 * p < TOK;
+                    load_scales(na[p], sA + (int64_t)(valid ? m : 0) * ldsA, b, b_last, valid);
+                }
+                load_scales(nb, rb, b, b_last, true);
+            };
+            fetch(b_first);
+            for (int b0 = 0; b0 < blocks && ok; b0 += 4) {
+                __syncwarp();
 #pragma unroll
-            for (int p = 0; p < PER; ++p)
-                if (lane + 32 * p < TOK)
+                for (int p = 0; p < PER; ++p)
+                    if (lane + 32 * p < TOK)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) my[i * TOK + lane + 32 * p] = na[p][i] * nb[i];
-            __syncwarp();
-            fetch(b_first + b0 + 4);
-            for (int i = 0; i < 4 && b0 + i < blocks; ++i) {
-                const int j = b0 + i, buf = j & 1;
-                // (one answer for the warp: its next steps are collective)
+                        for (int i = 0; i < 4; ++i) my[i * TOK + lane + 32 * p] = na[p][i] * nb[i];
+                __syncwarp();
+                fetch(b_first + b0 + 4);
+                for (int i = 0; i < 4 && b0 + i < blocks; ++i, ++j) {
+                    const int buf = j & 1;
+                    // (one answer for the warp: its next steps are collective)
                     if (!__all_sync(0xffffffffu, mbar_wait(tfull(buf), (j >> 1) & 1, abort_flag))) { ok = false; break; }
-                tc_fence_after();
-                constexpr int CH = TOK < 32 ? TOK : 32;
+                    tc_fence_after();
+                    constexpr int CH = TOK < 32 ? TOK : 32;
 #pragma unroll
-                for (int c = 0; c < TOK / CH; ++c) {
-                    uint32_t r[CH];
-                    if constexpr (CH == 16) tmem_ld_32x32b_x16(lanes + buf * TOK + c * CH, r);
-                    else tmem_ld_32x32b_x32(lanes + buf * TOK + c * CH, r);
-                    tmem_ld_wait();
-                    if (c == TOK / CH - 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(tempty(buf));
-                    }
-                    const float4 *s4 = reinterpret_cast<const float4 *>(my + i * TOK + c * CH);
+                    for (int c = 0; c < TOK / CH; ++c) {
+                        uint32_t r[CH];
+                        if constexpr (CH == 16) tmem_ld_32x32b_x16(lanes + buf * TOK + c * CH, r);
+                        else tmem_ld_32x32b_x32(lanes + buf * TOK + c * CH, r);
+                        tmem_ld_wait();
+                        if (c == TOK / CH - 1) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(tempty(buf));
+                        }
+                        const float4 *s4 = reinterpret_cast<const float4 *>(my + i * TOK + c * CH);
 #pragma unroll
-                    for (int u = 0; u < CH / 4; ++u) {
-                        const float4 s = s4[u];
-                        float *a = acc + c * CH + 4 * u;
-                        a[0] = fmaf(__uint_as_float(r[4 * u]), s.x, a[0]);
-                        a[1] = fmaf(__uint_as_float(r[4 * u + 1]), s.y, a[1]);
-                        a[2] = fmaf(__uint_as_float(r[4 * u + 2]), s.z, a[2]);
-                        a[3] = fmaf(__uint_as_float(r[4 * u + 3]), s.w, a[3]);
+                        for (int u = 0; u < CH / 4; ++u) {
+                            const float4 s = s4[u];
+                            float *a = acc + c * CH + 4 * u;
+                            a[0] = fmaf(__uint_as_float(r[4 * u]), s.x, a[0]);
+                            a[1] = fmaf(__uint_as_float(r[4 * u + 1]), s.y, a[1]);
+                            a[2] = fmaf(__uint_as_float(r[4 * u + 2]), s.z, a[2]);
+                            a[3] = fmaf(__uint_as_float(r[4 * u + 3]), s.w, a[3]);
+                        }
                     }
                 }
             }
-        }
-        // the last block's MMAs have read the stages: the sums may go over them
-        if (ok) {
+            if (!ok) break;
+            if (parts > 1) {
+                // the last block's MMAs have read the stages: the sums may go over them
 #pragma unroll
-            for (int i = 0; i < TOK; ++i) sums[i * BM + threadIdx.x] = acc[i];
+                for (int i = 0; i < TOK; ++i) sums[i * BM + threadIdx.x] = acc[i];
+            } else {
+                const int n = n0 + threadIdx.x;
+                if (n < N) {
+                    const float bv = bias ? __ldg(bias + n) : 0.0f;
+                    const int rows = M - m0;
+#pragma unroll
+                    for (int i = 0; i < TOK; ++i)
+                        if (i < rows) finish_store(C, (int64_t)(m0 + i) * ldc + n, acc[i], bv, epi);
+                }
+            }
         }
     }
     if (!ok) {
@@ -541,8 +595,8 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
     __syncthreads();
     if (*abort_flag) {
-        if (warp == 5 && lane == 0) {
-            mma_commit(drained);
+        if (warp == 5) {
+            if (elect_one()) mma_commit(drained);  // the lane that issued
             mbar_wait(drained, 0, nullptr, 400000000ll);
         }
         if (warp == 4 && lane == 0)
@@ -556,24 +610,27 @@ __global__ void __launch_bounds__(kSplitThreads)
         tc_fence_after();
         tmem_dealloc(tmem, P::TMEM);
     }
-    if (parts > 1) cluster.sync();
-    if (threadIdx.x < BM) {
-        const int n = n0 + threadIdx.x;
-        const int first = TOK * part / parts, last = min(TOK * (part + 1) / parts, M - m0);
-        const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
-        for (int m = first; m < last; ++m) {
-            float v = 0.0f;
-            for (int p = 0; p < parts; ++p) v += cluster.map_shared_rank(sums, p)[m * BM + threadIdx.x];
-            if (n < N) {
-                v = activate(v + bv, epi);
-                const int64_t at = (int64_t)(m0 + m) * ldc + n;
-                if (dtype == LONNX_DT_F32) static_cast<float *>(C)[at] = v;
-                else if (dtype == LONNX_DT_F16) static_cast<__half *>(C)[at] = from_f32<__half>(v);
-                else static_cast<__nv_bfloat16 *>(C)[at] = from_f32<__nv_bfloat16>(v);
+    if (parts > 1) {
+        cluster.sync();
+        const int tm = first_tile / tiles_n, n = (first_tile - tm * tiles_n) * BM + (int)threadIdx.x, m0 = tm * TOK;
+        if (threadIdx.x < BM) {
+            const int first = TOK * part / parts, last = min(TOK * (part + 1) / parts, M - m0);
+            const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
+            for (int m = first; m < last; m += 4) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+                for (int p = 0; p < parts; ++p) {
+                    const float *of = cluster.map_shared_rank(sums, p) + m * BM + threadIdx.x;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] += m + u < last ? of[u * BM] : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (n < N && m + u < last) finish_store(C, (int64_t)(m0 + m + u) * ldc + n, v[u], bv, epi);
             }
         }
+        cluster.sync();  // the others' shared memory is read until here
     }
-    if (parts > 1) cluster.sync();  // the others' shared memory is read until here
 }
 
 // K = 0: the bias through the activation
@@ -641,7 +698,7 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
     return LONNX_OK;
 }
 
-template <int TOK>
+template <int TOK, typename T>
 int launch_split(lonnx_ctx *ctx, const Problem &p) {
     using P = Split<TOK>;
     CUtensorMap ma, mb;
@@ -653,11 +710,12 @@ int launch_split(lonnx_ctx *ctx, const Problem &p) {
     if (tiles > (1 << 27)) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
     int parts = 1;
     while (parts < 8 && tiles * parts * 2 <= 2 * ctx->num_sms && nkb >= parts * 4) parts *= 2;
-    const int stages = std::min((nkb + parts - 1) / parts, P::MAX_STAGES), smem = P::smem(stages);
-    auto kernel = k_fp8_split<TOK>;
+    const int stages = std::min((nkb + parts - 1) / parts, P::MAX_STAGES), smem = P::smem(stages, parts);
+    const int64_t grid = parts > 1 ? tiles * parts : std::min<int64_t>(tiles, (int64_t)ctx->num_sms * P::PER_SM);
+    auto kernel = k_fp8_split<TOK, T>;
     LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * parts));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kSplitThreads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = ctx->stream;
@@ -668,8 +726,8 @@ int launch_split(lonnx_ctx *ctx, const Problem &p) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     ctx->launches++;
-    LONNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, p.C, p.dtype, p.ldc, p.M,
-                                  p.N, nkb, stages, p.epi, ctx->dev_flags));
+    LONNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, static_cast<T *>(p.C), p.ldc,
+                                  p.M, p.N, nkb, stages, p.epi, ctx->dev_flags));
     return LONNX_OK;
 }
 
@@ -683,12 +741,12 @@ int launch(lonnx_ctx *ctx, const Problem &p) {
         return LONNX_OK;
     }
     const int64_t tm = (p.M + BM - 1) / BM;
-    if (p.M <= 16) return launch_split<16>(ctx, p);
-    if (p.M <= 32) return launch_split<32>(ctx, p);
-    if (p.M <= 64) return launch_split<64>(ctx, p);
+    if (p.M <= 16) return launch_split<16, T>(ctx, p);
+    if (p.M <= 32) return launch_split<32, T>(ctx, p);
+    if (p.M <= 64) return launch_split<64, T>(ctx, p);
     if (tm * ((p.N + 255) / 256) >= ctx->num_sms) return launch_wide<256, T>(ctx, p);
     if (tm * ((p.N + 127) / 128) >= ctx->num_sms) return launch_wide<128, T>(ctx, p);
-    return launch_split<128>(ctx, p);
+    return launch_split<128, T>(ctx, p);
 }
 
 }  // namespace
