@@ -104,23 +104,27 @@ struct Wide {
 constexpr int kWideThreads = 640;
 constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 19;
 
-// Tiles in groups of 16 rows of tiles, column by column within a group, so
-// that the CTAs at work share both operands' tiles in L2.
+// Tiles in groups of `GROUP` rows of tiles, column by column within a group, so
+// that the CTAs at work share both operands' tiles in L2.  Where C leaves by
+// element stores, its rows do not start on sectors, and a group is one row of
+// tiles: two neighbours' halves of a sector meet in L2 (18651 x 17257 floats
+// written as tiles: 407 us in groups of 16, 351 row by row).
+template <int GROUP>
 __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int &tm, int &tn) {
-    constexpr int GROUP = 16;
     const int per = GROUP * tiles_n, g = t / per, first = g * GROUP;
     const int h = min(GROUP, tiles_m - first), r = t - g * per;
     tn = r / h;
     tm = first + r - tn * h;
 }
 
-template <int BN, typename T>
+template <int BN, typename T, bool BY_TMA>
 __global__ void __launch_bounds__(kWideThreads, 1)
     k_fp8_wide(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                const __grid_constant__ CUtensorMap mapC, const float *__restrict__ sA, int64_t ldsA,
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
-               int64_t ldc, int M, int N, int nkb, int epi, int by_tma, int *flags) {
+               int64_t ldc, int M, int N, int nkb, int epi, int *flags) {
     using W = Wide<BN>;
+    constexpr int GROUP = BY_TMA ? 16 : 1;
     constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *staging = base + S * W::STAGE;
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (lane == 0) {
                 for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                     int tm, tn;
-                    tile_at(t, tiles_m, tiles_n, tm, tn);
+                    tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
                     for (int b = 0; b < nkb; ++b, ++issued) {
                         const int s = issued % S;
                         if (!mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
                 const int set = SETS == 2 ? n & 1 : 0;
                 int tm, tn;
-                tile_at(t, tiles_m, tiles_n, tm, tn);
+                tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
                 const float *ra[4], *rb[NB];
                 float x[4], y[NB];
 #pragma unroll
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
             if (!ok) break;
             int tm, tn;
-            tile_at(t, tiles_m, tiles_n, tm, tn);
+            tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
             const int row0 = tm * BM + q * 32, col0 = tn * BN + part * COLS;
             auto finish = [&](int i) {  // 16 bytes of C from column i
                 constexpr int CN = 16 / (int)sizeof(T);
@@ -318,7 +322,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             };
             constexpr int CN = 16 / (int)sizeof(T);
             uint8_t *stage = staging + warp * 4096;
-            if (by_tma) {
+            if constexpr (BY_TMA) {
                 // 64 bytes of each of the warp's 32 rows at a time, through two
                 // buffers: one piece is computed while the last one leaves
                 constexpr int PIECE = 64 / (int)sizeof(T);
@@ -339,31 +343,46 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     }
                 }
             } else {
-                // 128 bytes of a row at a time by element stores, the warp along
-                // the row; 8 rows' loads and stores in flight
-                constexpr int PIECE = 128 / (int)sizeof(T);
+                // whole 64-column runs of a row by element stores, the warp along
+                // the row, 4 KB of rows at a time and 8 rows in flight
+                constexpr int ROW = COLS * (int)sizeof(T), TALL = 4096 / ROW;
+                const int rows = M - row0;
 #pragma unroll
-                for (int p = 0; p < COLS / PIECE; ++p) {
+                for (int h = 0; h < 32 / TALL; ++h) {
                     __syncwarp();
+                    if (h == 0) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = finish(p * PIECE + c * CN);
-                    __syncwarp();
-                    const int rows = M - row0;
-#pragma unroll
-                    for (int e0 = 0; e0 < PIECE; e0 += 32) {
-                        const int e = e0 + lane, col = col0 + p * PIECE + e;
-                        T *dst = C + (int64_t)row0 * ldc + col;
-#pragma unroll
-                        for (int r0 = 0; r0 < 32; r0 += 8) {
-                            T x[8];
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                x[r] = *reinterpret_cast<const T *>(stage + (r0 + r) * 128 + (((e / CN) ^ r) << 4) + e % CN * sizeof(T));
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                if (col < N && r0 + r < rows) dst[(int64_t)(r0 + r) * ldc] = x[r];
+                        for (int c = 0; c < COLS / CN; ++c) {
+                            const uint4 v = finish(c * CN);
+                            if (lane < TALL) *reinterpret_cast<uint4 *>(stage + lane * ROW + ((c ^ (lane & 7)) << 4)) = v;
                         }
+                    } else if (lane >= TALL) {
+#pragma unroll
+                        for (int c = 0; c < COLS / CN; ++c) {
+                            T out[CN];
+#pragma unroll
+                            for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[c * CN + u]);
+                            *reinterpret_cast<uint4 *>(stage + (lane - TALL) * ROW + ((c ^ (lane & 7)) << 4)) =
+                                *reinterpret_cast<const uint4 *>(out);
+                        }
+                    }
+                    __syncwarp();
+                    T *dst = C + (int64_t)(row0 + h * TALL) * ldc + col0 + lane;
+#pragma unroll
+                    for (int r0 = 0; r0 < TALL; r0 += 8) {
+                        T x[8][COLS / 32];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+#pragma unroll
+                            for (int e = 0; e < COLS / 32; ++e) {
+                                const int i = lane + 32 * e;
+                                x[r][e] = *reinterpret_cast<const T *>(stage + (r0 + r) * ROW + (((i / CN) ^ r) << 4) + i % CN * sizeof(T));
+                            }
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+#pragma unroll
+                            for (int e = 0; e < COLS / 32; ++e)
+                                if (col0 + lane + 32 * e < N && h * TALL + r0 + r < rows) dst[(int64_t)(r0 + r) * ldc + 32 * e] = x[r][e];
                     }
                 }
             }
@@ -671,16 +690,15 @@ struct Problem {
     int dtype, M, N, K, epi;
 };
 
-template <int BN, typename T>
+template <int BN, typename T, bool BY_TMA>
 int launch_wide(lonnx_ctx *ctx, const Problem &p) {
     using W = Wide<BN>;
     CUtensorMap ma, mb, mc;
     int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, BM);
     if (!rc) rc = tile_map(&mb, p.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.ldb, BN);
     if (rc) return rc;
-    const bool by_tma = ((uintptr_t)p.C & 15) == 0 && p.ldc * (int64_t)sizeof(T) % 16 == 0;
-    mc = ma;  // unused unless by_tma
-    if (by_tma) {
+    mc = ma;  // unused unless BY_TMA
+    if (BY_TMA) {
         const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : p.dtype == LONNX_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -689,13 +707,19 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
     }
     const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
     if (tiles >= (1ll << 31) - 1024) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
-    auto kernel = k_fp8_wide<BN, T>;
+    auto kernel = k_fp8_wide<BN, T, BY_TMA>;
     LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM));
     kernel<<<(unsigned)std::min<int64_t>(tiles, ctx->num_sms), kWideThreads, W::SMEM, ctx->stream>>>(
         ma, mb, mc, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, static_cast<T *>(p.C), p.ldc, p.M, p.N, (p.K + KB - 1) / KB,
-        p.epi, by_tma, ctx->dev_flags);
+        p.epi, ctx->dev_flags);
     LONNX_CHECK_LAUNCH(ctx);
     return LONNX_OK;
+}
+
+template <int BN, typename T>
+int launch_wide(lonnx_ctx *ctx, const Problem &p) {
+    const bool by_tma = ((uintptr_t)p.C & 15) == 0 && p.ldc * (int64_t)sizeof(T) % 16 == 0;
+    return by_tma ? launch_wide<BN, T, true>(ctx, p) : launch_wide<BN, T, false>(ctx, p);
 }
 
 template <int TOK, typename T>
