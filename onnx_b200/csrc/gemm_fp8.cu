@@ -74,9 +74,8 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 // CTA = 20 warps, one per SM, walking tiles of 128 x BN:
 //   warps 0-15   drain: each thread one row x 64 columns in registers (four
 //                warps a scheduler: the TMEM loads of one hide behind the FMAs
-//                of the others); then the epilogue, 64 bytes of a row at a time
-//                through twice 2 KB of shared memory per warp and out by TMA
-//                (or, where rows of C do not start on 16 bytes, by element
+//                of the others); then the epilogue, 128 bytes of a row at a
+//                time through 4 KB of shared memory per warp and out by TMA (or, where rows of C do not start on 16 bytes, by element
 //                stores that coalesce along rows)
 //   warp 16      TMA producer
 //   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM): waits and
@@ -291,55 +290,58 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             int tm, tn;
             tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
             const int row0 = tm * BM + q * 32, col0 = tn * BN + part * COLS;
-            auto finish = [&](int i) {  // 16 bytes of C from column i
-                constexpr int CN = 16 / (int)sizeof(T);
+            // bias and activation of columns [i, i + 32), in place
+            auto finish = [&](int i) {
                 if (bias) {
                     if (bias4 && col0 + COLS <= N) {
 #pragma unroll
-                        for (int u = 0; u < CN; u += 4) {
-                            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + col0 + i + u));
-                            acc[i + u] += v.x;
-                            acc[i + u + 1] += v.y;
-                            acc[i + u + 2] += v.z;
-                            acc[i + u + 3] += v.w;
+                        for (int u = i; u < i + 32; u += 4) {
+                            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + col0 + u));
+                            acc[u] += v.x;
+                            acc[u + 1] += v.y;
+                            acc[u + 2] += v.z;
+                            acc[u + 3] += v.w;
                         }
                     } else {
 #pragma unroll
-                        for (int u = 0; u < CN; ++u) acc[i + u] += __ldg(bias + min(col0 + i + u, N - 1));
+                        for (int u = i; u < i + 32; ++u) acc[u] += __ldg(bias + min(col0 + u, N - 1));
                     }
                 }
                 if (epi == LONNX_EPI_RELU) {
 #pragma unroll
-                    for (int u = 0; u < CN; ++u) acc[i + u] = activate(acc[i + u], LONNX_EPI_RELU);
+                    for (int u = i; u < i + 32; ++u) acc[u] = activate(acc[u], LONNX_EPI_RELU);
                 } else if (epi == LONNX_EPI_GELU_ERF) {
 #pragma unroll
-                    for (int u = 0; u < CN; ++u) acc[i + u] = lonnx_gelu_fast(acc[i + u]);
+                    for (int u = i; u < i + 32; ++u) acc[u] = lonnx_gelu_fast(acc[u]);
                 }
+            };
+            constexpr int CN = 16 / (int)sizeof(T);
+            auto pack = [&](int i) {  // 16 bytes of C from column i
                 T out[CN];
 #pragma unroll
                 for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[i + u]);
                 return *reinterpret_cast<const uint4 *>(out);
             };
-            constexpr int CN = 16 / (int)sizeof(T);
             uint8_t *stage = staging + warp * 4096;
             if constexpr (BY_TMA) {
-                // 64 bytes of each of the warp's 32 rows at a time, through two
-                // buffers: one piece is computed while the last one leaves
-                constexpr int PIECE = 64 / (int)sizeof(T);
+                // 128 bytes of each of the warp's 32 rows at a time: one piece is
+                // computed in registers while the last one leaves shared memory
+                constexpr int PIECE = 128 / (int)sizeof(T);
 #pragma unroll
                 for (int p = 0; p < COLS / PIECE; ++p) {
-                    uint8_t *buf = stage + (p & 1) * 2048;
-                    if (lane == 0) bulk_wait_group_read1();
+#pragma unroll
+                    for (int i = p * PIECE; i < (p + 1) * PIECE; i += 32) finish(i);
+                    if (lane == 0) bulk_wait_group_read0();
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)  // 16-byte chunks of this lane's row, 64B-swizzled
-                        *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = finish(p * PIECE + c * CN);
+                    for (int c = 0; c < 8; ++c)  // 16-byte chunks of this lane's row, 128B-swizzled
+                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack(p * PIECE + c * CN);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
-                        const int col = col0 + p * PIECE;
-                        if (col < N && row0 < M) tma_store_2d(&mapC, smem_u32(buf), col, row0);
-                        bulk_commit_group();  // (an empty group keeps the count)
+                    const int col = col0 + p * PIECE;
+                    if (lane == 0 && col < N && row0 < M) {
+                        tma_store_2d(&mapC, smem_u32(stage), col, row0);
+                        bulk_commit_group();
                     }
                 }
             } else {
@@ -352,19 +354,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     __syncwarp();
                     if (h == 0) {
 #pragma unroll
-                        for (int c = 0; c < COLS / CN; ++c) {
-                            const uint4 v = finish(c * CN);
-                            if (lane < TALL) *reinterpret_cast<uint4 *>(stage + lane * ROW + ((c ^ (lane & 7)) << 4)) = v;
-                        }
-                    } else if (lane >= TALL) {
+                        for (int i = 0; i < COLS; i += 32) finish(i);
+                    }
+                    if (lane / TALL == h) {
 #pragma unroll
-                        for (int c = 0; c < COLS / CN; ++c) {
-                            T out[CN];
-#pragma unroll
-                            for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[c * CN + u]);
-                            *reinterpret_cast<uint4 *>(stage + (lane - TALL) * ROW + ((c ^ (lane & 7)) << 4)) =
-                                *reinterpret_cast<const uint4 *>(out);
-                        }
+                        for (int c = 0; c < COLS / CN; ++c)
+                            *reinterpret_cast<uint4 *>(stage + lane % TALL * ROW + ((c ^ (lane & 7)) << 4)) = pack(c * CN);
                     }
                     __syncwarp();
                     T *dst = C + (int64_t)(row0 + h * TALL) * ldc + col0 + lane;
@@ -664,19 +659,17 @@ __global__ void k_fp8_no_columns(const float *__restrict__ bias, T *__restrict__
 
 // ---- host side ------------------------------------------------------------------
 
-// row-major [rows, cols] of es-byte elements, leading dimension ld elements, box of
-// row_bytes (128 or 64, swizzled alike) x box_rows
+// row-major [rows, cols] of es-byte elements, leading dimension ld elements, box of 128 bytes x box_rows
 int tile_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int es, int64_t rows, int64_t cols,
-             int64_t ld, int box_rows, int row_bytes = 128) {
+             int64_t ld, int box_rows) {
     lonnx::tc::EncodeTiledFn enc = lonnx::tc::encode_tiled();
     if (!enc) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled unavailable");
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
-    const cuuint32_t box[2] = {(cuuint32_t)(row_bytes / es), (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return lonnx::set_error(LONNX_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return LONNX_OK;
@@ -702,7 +695,7 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
         const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : p.dtype == LONNX_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        rc = tile_map(&mc, p.C, type, (int)sizeof(T), p.M, p.N, p.ldc, 32, 64);
+        rc = tile_map(&mc, p.C, type, (int)sizeof(T), p.M, p.N, p.ldc, 32);
         if (rc) return rc;
     }
     const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
