@@ -11,7 +11,7 @@
 //
 // Two kernels.  k_fp8_wide: tiles of 128 rows of A x BN rows of B, for
 // problems that fill the GPU with them.  k_fp8_split: B's rows as the tensor
-// core's 128 and 16 to 128 rows of A as its columns, K split over the CTAs of
+// core's 128 and 16 to 64 rows of A as its columns, K split over the CTAs of
 // a cluster that add their sums over distributed shared memory: for few rows,
 // where the weights' bytes and the latency count.  Neither needs a workspace.
 #include <cooperative_groups.h>
@@ -46,6 +46,50 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 __device__ __forceinline__ float activate(float v, int epi) {
     if (epi == LONNX_EPI_RELU) return v > 0.0f ? v : 0.0f;  // NaN gives 0, as lonnx_gemm_f32's
     return epi == LONNX_EPI_GELU_ERF ? lonnx_gelu_fast(v) : v;
+}
+
+// lonnx_gelu_fast of two values, with one reciprocal for both (1 / d0 = d1 / (d0
+// d1)) and the multiplications and FMAs in pairs.  The clamp keeps the product
+// finite; beyond it erf is +-1, and the last line has infinities and NaN.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void gelu2(float &x, float &y) {
+    const uint64_t a = pack2(fminf(fabsf(x) * 0.707106769084930419921875f, 1e10f),
+                             fminf(fabsf(y) * 0.707106769084930419921875f, 1e10f));
+    const float2 d = unpack2(fma2(pack2(0.3275911f, 0.3275911f), a, pack2(1.0f, 1.0f)));
+    float r, e0, e1;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d.x * d.y));
+    const uint64_t t = pack2(r * d.y, r * d.x);
+    const float2 q = unpack2(mul2(mul2(a, a), pack2(-1.44269504102162933349609375f, -1.44269504102162933349609375f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(q.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(q.y));
+    uint64_t p = fma2(pack2(-1.061405429f, -1.061405429f), t, pack2(1.453152027f, 1.453152027f));
+    p = fma2(p, t, pack2(-1.421413741f, -1.421413741f));
+    p = fma2(p, t, pack2(0.284496736f, 0.284496736f));
+    p = fma2(p, t, pack2(-0.254829592f, -0.254829592f));
+    const float2 erf = unpack2(fma2(mul2(p, t), pack2(e0, e1), pack2(1.0f, 1.0f)));
+    const uint64_t h = mul2(pack2(x, y), pack2(0.5f, 0.5f));
+    const float2 g = unpack2(fma2(h, pack2(copysignf(erf.x, x), copysignf(erf.y, y)), h));
+    x = g.x;
+    y = g.y;
 }
 
 // D[tmem] (+)= A[smem desc] x B[smem desc], kind::f8f6f4 (32 columns of K), one CTA
@@ -312,7 +356,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     for (int u = i; u < i + 32; ++u) acc[u] = activate(acc[u], LONNX_EPI_RELU);
                 } else if (epi == LONNX_EPI_GELU_ERF) {
 #pragma unroll
-                    for (int u = i; u < i + 32; ++u) acc[u] = lonnx_gelu_fast(acc[u]);
+                    for (int u = i; u < i + 32; u += 2) gelu2(acc[u], acc[u + 1]);
                 }
             };
             constexpr int CN = 16 / (int)sizeof(T);
@@ -423,11 +467,16 @@ struct Split {
     static constexpr int STAGE = kTile + TOK * KB;
     static constexpr int TMEM = 2 * TOK < 32 ? 32 : 2 * TOK;
     static constexpr int SCALES = 4 * 4 * TOK * 4;  // 4 warps x 4 blocks
-    static constexpr int MAX_STAGES = TOK == 16 ? 4 : 3;
+    static constexpr int MAX_STAGES = 12;
     static constexpr int BARS = 2 * MAX_STAGES + 5;
-    static constexpr int PER_SM = TOK == 128 ? 2 : 3;  // by shared memory
+    static constexpr int PER_SM = TOK == 64 ? 2 : 3;  // CTAs, by registers
     static int smem(int stages, int parts) {
         return std::max(stages * STAGE, parts > 1 ? TOK * BM * 4 : 0) + SCALES + BARS * 8 + 8;
+    }
+    // as many stages as fit with `per_sm` CTAs on an SM: few CTAs have to keep more bytes in flight each
+    static int stages(int blocks, int per_sm) {
+        const int room = 227 * 1024 / per_sm - 1024 - SCALES - BARS * 8 - 8;
+        return std::max(1, std::min({blocks, room / STAGE, MAX_STAGES}));
     }
 };
 
@@ -437,7 +486,7 @@ __device__ __forceinline__ void finish_store(T *C, int64_t at, float v, float bi
 }
 
 template <int TOK, typename T>
-__global__ void __launch_bounds__(kSplitThreads, TOK == 128 ? 1 : TOK == 64 ? 2 : 3)
+__global__ void __launch_bounds__(kSplitThreads, Split<TOK>::PER_SM)
     k_fp8_split(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                 const float *__restrict__ sA, int64_t ldsA, const float *__restrict__ sB, int64_t ldsB,
                 const float *__restrict__ bias, T *__restrict__ C, int64_t ldc, int M, int N, int nkb, int stages,
@@ -716,7 +765,7 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
 }
 
 template <int TOK, typename T>
-int launch_split(lonnx_ctx *ctx, const Problem &p) {
+int launch_split(lonnx_ctx *ctx, const Problem &p, int parts) {
     using P = Split<TOK>;
     CUtensorMap ma, mb;
     int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, TOK);
@@ -725,10 +774,9 @@ int launch_split(lonnx_ctx *ctx, const Problem &p) {
     const int nkb = (p.K + KB - 1) / KB;
     const int64_t tiles = (int64_t)((p.N + BM - 1) / BM) * ((p.M + TOK - 1) / TOK);
     if (tiles > (1 << 27)) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 2 * ctx->num_sms && nkb >= parts * 4) parts *= 2;
-    const int stages = std::min((nkb + parts - 1) / parts, P::MAX_STAGES), smem = P::smem(stages, parts);
     const int64_t grid = parts > 1 ? tiles * parts : std::min<int64_t>(tiles, (int64_t)ctx->num_sms * P::PER_SM);
+    const int per_sm = (int)std::min<int64_t>(P::PER_SM, (grid + ctx->num_sms - 1) / ctx->num_sms);
+    const int stages = P::stages((nkb + parts - 1) / parts, per_sm), smem = P::smem(stages, parts);
     auto kernel = k_fp8_split<TOK, T>;
     LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
@@ -748,6 +796,52 @@ int launch_split(lonnx_ctx *ctx, const Problem &p) {
     return LONNX_OK;
 }
 
+// Which kernel and tile: the least time by a model of both, in microseconds.
+// Wide tiles take a time per block and one per epilogue, in rounds over the
+// SMs; split ones a time per block, an addition of sums per cluster, and more
+// where SMs get several CTAs.  Either takes at least its tiles' bytes through
+// L2.  The constants are fitted to 24 shapes from 1 x 1000 x 8000 to 1000 x 20000
+// x 300 in all 14 variants; the choice is within 3.5% of the best of them on
+// average (e.g. 1 x 4096 x 4096: split 16 by 4 at 6.2 us, unsplit 10.7, wide
+// 13.5; 777 x 1000 x 1111: wide 128 7.6, wide 256 9.9, split 64 9.1; 256 x 4096 x
+// 4096: wide 128 15.3, split 64 18.3).
+struct Choice {
+    int width, parts;  // 256, 128: wide tiles; 64, 32, 16: rows of A of a split tile
+};
+Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const double l2 = 7.5e6;  // bytes a microsecond
+    const int64_t nkb = up(K, KB);
+    Choice best{128, 1};
+    double least = 1e30;
+    const auto offer = [&](int width, int parts, double t) {
+        if (t < least) {
+            least = t;
+            best = {width, parts};
+        }
+    };
+    for (int bn : {256, 128}) {
+        const int64_t tiles = up(M, BM) * up(N, bn), rounds = up(tiles, sms);
+        const double block = bn == 256 ? 0.58 : tiles > sms ? 0.39 : 0.31, epilogue = bn == 256 ? 2.3 : 1.2;
+        offer(bn, 1, std::max(rounds * (nkb * block + epilogue), tiles * nkb * double(kTile + bn * KB) / l2));
+    }
+    // CTAs that run at once in clusters of 1, 2, 4, 8 (a GPC has 16 to 18 SMs)
+    const double at_once[4] = {1.0, 0.98, 0.89, 0.70};
+    for (int tok : {16, 32, 64}) {
+        const int64_t tiles = up(N, BM) * up(M, tok);
+        const double block = tok == 16 ? 0.235 : tok == 32 ? 0.265 : 0.33, epilogue = tok == 64 ? 0.6 : 0.3;
+        for (int i = 0; i < 4; ++i) {
+            const int parts = 1 << i;
+            if (parts > std::max<int64_t>(1, nkb / 2)) break;
+            const int64_t rounds = up(tiles * parts, (int64_t)(sms * at_once[i]));
+            const double t = up(nkb, parts) * block * (1 + 0.75 * (rounds - 1)) + epilogue * rounds;
+            const double join = parts > 1 ? 1.4 + 2.0 * (rounds - 1) : 0.0;
+            offer(tok, parts, std::max(t, tiles * nkb * double(kTile + tok * KB) / l2) + join);
+        }
+    }
+    return best;
+}
+
 template <typename T>
 int launch(lonnx_ctx *ctx, const Problem &p) {
     if (p.K == 0) {
@@ -757,13 +851,14 @@ int launch(lonnx_ctx *ctx, const Problem &p) {
         LONNX_CHECK_LAUNCH(ctx);
         return LONNX_OK;
     }
-    const int64_t tm = (p.M + BM - 1) / BM;
-    if (p.M <= 16) return launch_split<16, T>(ctx, p);
-    if (p.M <= 32) return launch_split<32, T>(ctx, p);
-    if (p.M <= 64) return launch_split<64, T>(ctx, p);
-    if (tm * ((p.N + 255) / 256) >= ctx->num_sms) return launch_wide<256, T>(ctx, p);
-    if (tm * ((p.N + 127) / 128) >= ctx->num_sms) return launch_wide<128, T>(ctx, p);
-    return launch_split<128, T>(ctx, p);
+    const Choice c = choose(p.M, p.N, p.K, ctx->num_sms);
+    switch (c.width) {
+        case 256: return launch_wide<256, T>(ctx, p);
+        case 128: return launch_wide<128, T>(ctx, p);
+        case 64: return launch_split<64, T>(ctx, p, c.parts);
+        case 32: return launch_split<32, T>(ctx, p, c.parts);
+        default: return launch_split<16, T>(ctx, p, c.parts);
+    }
 }
 
 }  // namespace
