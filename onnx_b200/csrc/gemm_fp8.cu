@@ -750,7 +750,11 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
     const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
     if (tiles >= (1ll << 31) - 1024) return lonnx::set_error(LONNX_E_UNSUPPORTED, "gemm_fp8: too many tiles");
     auto kernel = k_fp8_wide<BN, T, BY_TMA>;
-    LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM));
+    static bool attr_set[64] = {false};
+    if (!attr_set[ctx->device & 63]) {
+        LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM));
+        attr_set[ctx->device & 63] = true;
+    }
     kernel<<<(unsigned)std::min<int64_t>(tiles, ctx->num_sms), kWideThreads, W::SMEM, ctx->stream>>>(
         ma, mb, mc, p.sA, p.ldsA, p.sB, p.ldsB, p.bias, static_cast<T *>(p.C), p.ldc, p.M, p.N, (p.K + KB - 1) / KB,
         p.epi, ctx->dev_flags);
@@ -778,7 +782,11 @@ int launch_split(lonnx_ctx *ctx, const Problem &p, int parts) {
     const int per_sm = (int)std::min<int64_t>(P::PER_SM, (grid + ctx->num_sms - 1) / ctx->num_sms);
     const int stages = P::stages((nkb + parts - 1) / parts, per_sm), smem = P::smem(stages, parts);
     auto kernel = k_fp8_split<TOK, T>;
-    LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static bool attr_set[64] = {false};
+    if (!attr_set[ctx->device & 63]) {
+        LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        attr_set[ctx->device & 63] = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kSplitThreads);

@@ -482,8 +482,11 @@ int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (parts > 8)
-        LONNX_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    static bool attr_set[64] = {false};
+    if (!attr_set[ctx->device & 63]) {
+        LONNX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attr_set[ctx->device & 63] = true;
+    }
     ctx->launches++;
     LONNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, x, g));
     return LONNX_OK;

@@ -25,16 +25,20 @@ from .tensor import BFLOAT16, FLOAT8E4M3, ONNX_DTYPE, Context, DeviceTensor
 
 BLOCK = 128          # columns of a quantisation block, and rows of a weight's
 MAX_ALTERNATIVES = 32
-FLOAT_TYPES = (np.dtype(np.float32), np.dtype(np.float16), BFLOAT16)
+F32, I64 = (np.dtype(np.float32),), (np.dtype(np.int64),)
+FP8 = (FLOAT8E4M3,)
+FLOAT_TYPES = F32 + (np.dtype(np.float16), BFLOAT16)
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2}
 
-
-def _ceil(a: int, b: int) -> int:
-    return -(-a // b)
+_quantize, _gemm, _logprobs = N.lib.lonnx_quantize_fp8, N.lib.lonnx_gemm_fp8, N.lib.lonnx_token_logprobs
 
 
-def _need(t, what: str, ctx: Context, dtypes, shape=None) -> DeviceTensor:
-    """``t`` if it is a tensor of this context's device, of these types and shape."""
+def _need(t, what: str, ctx: Context, dtypes, shape=None) -> None:
+    """Refuses a ``t`` that is not a tensor on this context's stream, of these
+    types and of this shape (None: any matrix)."""
+    if isinstance(t, DeviceTensor) and t.ctx is ctx and t.dtype in dtypes and \
+            (t.shape == shape if shape is not None else len(t.shape) == 2):
+        return
     if not isinstance(t, DeviceTensor):
         raise TypeError(f"{what}: expected a DeviceTensor, got {type(t).__name__}")
     if t.ctx is not ctx and (t.ctx.device != ctx.device or t.ctx.stream != ctx.stream):
@@ -45,7 +49,6 @@ def _need(t, what: str, ctx: Context, dtypes, shape=None) -> DeviceTensor:
         raise ValueError(f"{what}: expected a matrix, got shape {t.shape}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: expected shape {shape}, got {t.shape}")
-    return t
 
 
 @dataclass
@@ -68,23 +71,23 @@ def quantize_fp8(x: DeviceTensor, block_rows: int = 1, out=None) -> Fp8Matrix:
     per 1 x 128 (``block_rows=1``) or 128 x 128 block.  ``out``: (q, scale) to
     write; otherwise they are made, with rows of ``q`` 16-byte aligned as
     ``matmul_fp8`` needs them."""
-    if not isinstance(x, DeviceTensor):
-        raise TypeError(f"x: expected a DeviceTensor, got {type(x).__name__}")
-    ctx = x.ctx
+    ctx = getattr(x, "ctx", None)
     _need(x, "x", ctx, FLOAT_TYPES)
-    if block_rows not in (1, BLOCK):
+    if block_rows != 1 and block_rows != BLOCK:
         raise ValueError(f"block_rows: 1 or {BLOCK}, got {block_rows}")
     rows, cols = x.shape
-    scales = (_ceil(rows, block_rows), _ceil(cols, BLOCK))
+    scales = (-(-rows // block_rows), -(-cols // BLOCK))
     if out is None:
-        out = (DeviceTensor(ctx, (rows, _ceil(cols, 16) * 16), FLOAT8E4M3), DeviceTensor(ctx, scales, np.float32))
+        out = (DeviceTensor(ctx, (rows, -(-cols // 16) * 16), FLOAT8E4M3), DeviceTensor(ctx, scales, F32[0]))
     q, scale = out
-    _need(q, "out q", ctx, (FLOAT8E4M3,))
-    _need(scale, "out scale", ctx, (np.dtype(np.float32),), scales)
-    if q.shape[0] != rows or q.shape[1] < cols:
+    _need(q, "out q", ctx, FP8)
+    _need(scale, "out scale", ctx, F32, scales)
+    ldq = q.shape[1]
+    if q.shape[0] != rows or ldq < cols:
         raise ValueError(f"out q: expected [{rows}, >= {cols}], got {q.shape}")
-    N.check(N.lib.lonnx_quantize_fp8(ctx.handle, x.ptr, ONNX_DTYPE[x.dtype], rows, cols, cols, block_rows, q.ptr,
-                                     q.shape[1], scale.ptr, scales[1]))
+    rc = _quantize(ctx.handle, x.ptr, ONNX_DTYPE[x.dtype], rows, cols, cols, block_rows, q.ptr, ldq, scale.ptr, scales[1])
+    if rc:
+        N.check(rc)
     return Fp8Matrix(q, scale, cols, block_rows)
 
 
@@ -96,26 +99,28 @@ def matmul_fp8(a: Fp8Matrix, w: Fp8Matrix, bias: DeviceTensor | None = None, act
     ctx = a.q.ctx
     if a.block_rows != 1 or w.block_rows != BLOCK:
         raise ValueError(f"blocks of {a.block_rows} and {w.block_rows} rows: a needs 1, w {BLOCK}")
-    if a.cols != w.cols:
-        raise ValueError(f"a has {a.cols} columns, w {w.cols}")
+    k = a.cols
+    if k != w.cols:
+        raise ValueError(f"a has {k} columns, w {w.cols}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation: None, 'relu' or 'gelu', got {activation!r}")
-    m, n, k = a.rows, w.rows, a.cols
-    kb = _ceil(k, BLOCK)
-    f32 = np.dtype(np.float32)
-    for x, what, rows in ((a, "a", m), (w, "w", _ceil(n, BLOCK))):
-        _need(x.q, what, ctx, (FLOAT8E4M3,))
-        _need(x.scale, f"{what} scale", ctx, (f32,), (rows, kb))
-        if x.q.shape[1] < k or x.q.shape[1] % 16:
-            raise ValueError(f"{what}: rows of {x.q.shape[1]} bytes (at least {k}, a multiple of 16)")
+    _need(a.q, "a", ctx, FP8)
+    _need(w.q, "w", ctx, FP8)
+    (m, lda), (n, ldw) = a.q.shape, w.q.shape
+    kb = -(-k // BLOCK)
+    _need(a.scale, "a scale", ctx, F32, (m, kb))
+    _need(w.scale, "w scale", ctx, F32, (-(-n // BLOCK), kb))
+    if lda < k or ldw < k or lda % 16 or ldw % 16:
+        raise ValueError(f"a and w: rows of {lda} and {ldw} bytes (at least {k}, multiples of 16)")
     if bias is not None:
-        _need(bias, "bias", ctx, (f32,), (n,))
+        _need(bias, "bias", ctx, F32, (n,))
     if out is None:
         out = DeviceTensor(ctx, (m, n), dtype)
     _need(out, "out", ctx, FLOAT_TYPES, (m, n))
-    N.check(N.lib.lonnx_gemm_fp8(ctx.handle, a.q.ptr, a.q.shape[1], a.scale.ptr, kb, w.q.ptr, w.q.shape[1],
-                                 w.scale.ptr, kb, bias.ptr if bias is not None else None, out.ptr,
-                                 ONNX_DTYPE[out.dtype], n, m, n, k, ACTIVATIONS[activation]))
+    rc = _gemm(ctx.handle, a.q.ptr, lda, a.scale.ptr, kb, w.q.ptr, ldw, w.scale.ptr, kb,
+               None if bias is None else bias.ptr, out.ptr, ONNX_DTYPE[out.dtype], n, m, n, k, ACTIVATIONS[activation])
+    if rc:
+        N.check(rc)
     return out
 
 
@@ -127,9 +132,7 @@ def token_logprobs(logits: DeviceTensor, targets: DeviceTensor | None = None, k:
     and ``top_id`` (int64).  ``vocab``: the columns to read, where the rows are
     wider than the vocabulary.  ``out``: tensors to write, by the same names;
     one that is left out is not computed (the alternatives come in pairs)."""
-    if not isinstance(logits, DeviceTensor):
-        raise TypeError(f"logits: expected a DeviceTensor, got {type(logits).__name__}")
-    ctx = logits.ctx
+    ctx = getattr(logits, "ctx", None)
     _need(logits, "logits", ctx, FLOAT_TYPES)
     rows, ld = logits.shape
     vocab = ld if vocab is None else int(vocab)
@@ -137,27 +140,26 @@ def token_logprobs(logits: DeviceTensor, targets: DeviceTensor | None = None, k:
         raise ValueError(f"vocab: 1 to {ld}, got {vocab}")
     if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
         raise ValueError(f"k: 0 to {min(MAX_ALTERNATIVES, vocab)}, got {k}")
-    f32, i64 = np.dtype(np.float32), np.dtype(np.int64)
+    each, top = (rows,), (rows, k)
     if targets is not None:
-        _need(targets, "targets", ctx, (i64,), (rows,))
-    kinds = {"entropy": ((rows,), f32)}
-    if targets is not None:
-        kinds["logprob"] = ((rows,), f32)
-    if k:
-        kinds["top_logprob"], kinds["top_id"] = ((rows, k), f32), ((rows, k), i64)
+        _need(targets, "targets", ctx, I64, each)
     if out is None:
-        out = {name: DeviceTensor(ctx, shape, dt) for name, (shape, dt) in kinds.items()}
+        out = {"entropy": DeviceTensor(ctx, each, F32[0])}
+        if targets is not None:
+            out["logprob"] = DeviceTensor(ctx, each, F32[0])
+        if k:
+            out["top_logprob"], out["top_id"] = DeviceTensor(ctx, top, F32[0]), DeviceTensor(ctx, top, I64[0])
+    ptr = dict.fromkeys(("logprob", "entropy", "top_logprob", "top_id"))
     for name, t in out.items():
-        if name not in kinds:
-            raise ValueError(f"out: {name!r} is not an output of this call ({', '.join(sorted(kinds))})")
-        _need(t, f"out {name}", ctx, (kinds[name][1],), kinds[name][0])
-    if k and not ("top_logprob" in out and "top_id" in out):
+        if name not in ptr or (name == "logprob" and targets is None) or (name[0] == "t" and not k):
+            raise ValueError(f"out: {name!r} is not an output of this call")
+        _need(t, name, ctx, I64 if name == "top_id" else F32, top if name[0] == "t" else each)
+        ptr[name] = t.ptr
+    if k and (ptr["top_logprob"] is None or ptr["top_id"] is None):
         raise ValueError("out: top_logprob and top_id are both needed with k > 0")
-
-    def ptr(name):
-        return out[name].ptr if name in out else None
-
-    N.check(N.lib.lonnx_token_logprobs(ctx.handle, logits.ptr, ONNX_DTYPE[logits.dtype], rows, vocab, ld,
-                                       targets.ptr if targets is not None else None, float(temperature),
-                                       ptr("logprob"), ptr("entropy"), k, ptr("top_logprob"), ptr("top_id")))
+    rc = _logprobs(ctx.handle, logits.ptr, ONNX_DTYPE[logits.dtype], rows, vocab, ld,
+                   None if targets is None else targets.ptr, temperature, ptr["logprob"], ptr["entropy"], k,
+                   ptr["top_logprob"], ptr["top_id"])
+    if rc:
+        N.check(rc)
     return out

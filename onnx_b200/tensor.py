@@ -66,23 +66,36 @@ class Context:
             self.handle = None
 
 
+class _Allocation:
+    """Memory of a context's allocator, given back with its last tensor."""
+
+    def __init__(self, ctx: Context, nbytes: int):
+        p = ctypes.c_void_p()
+        N.check(N.lib.lonnx_malloc(ctx.handle, max(nbytes, 1), ctypes.byref(p)))
+        self.ctx, self.ptr = ctx, p.value
+
+    def __del__(self):
+        try:
+            if self.ptr and self.ctx.handle:
+                N.lib.lonnx_free(self.ctx.handle, self.ptr)
+        except Exception:
+            pass
+
+
 class DeviceTensor:
     """A dense tensor in device memory (float32 activations, int64 indices)."""
 
+    name = None
+
     def __init__(self, ctx: Context, shape, dtype, ptr=None, owner=None):
         self.ctx = ctx
-        self.shape = tuple(int(s) for s in shape)
+        self.shape = tuple(map(int, shape))
         self.dtype = np.dtype(dtype)
-        self.name = None
-        self._owner = owner
         if ptr is None:
-            p = ctypes.c_void_p()
-            N.check(N.lib.lonnx_malloc(ctx.handle, max(self.nbytes, 1), ctypes.byref(p)))
-            self.ptr = p.value
-            self._owns = True
-        else:
-            self.ptr = ptr
-            self._owns = False
+            owner = _Allocation(ctx, self.nbytes)
+            ptr = owner.ptr
+        self.ptr = ptr
+        self._owner = owner
 
     @property
     def size(self) -> int:
@@ -123,13 +136,6 @@ class DeviceTensor:
         if int(np.prod(shape)) != self.size:
             raise ValueError(f"cannot reshape {self.shape} to {tuple(shape)}")
         return DeviceTensor(self.ctx, shape, self.dtype, ptr=self.ptr, owner=self)
-
-    def __del__(self):
-        try:
-            if self._owns and self.ptr and self.ctx.handle:
-                N.lib.lonnx_free(self.ctx.handle, self.ptr)
-        except Exception:
-            pass
 
     def __repr__(self):
         return f"DeviceTensor(shape={self.shape}, dtype={self.dtype}, device={self.ctx.device})"
