@@ -37,6 +37,9 @@
 
 namespace cg = cooperative_groups;
 
+#ifndef LB
+#define LB 3
+#endif
 namespace {
 
 constexpr int kMaxTop = 32;  // one list entry per lane
@@ -138,6 +141,75 @@ __device__ __forceinline__ uint64_t merge_desc(uint64_t a, uint64_t b, int lane)
     return key;
 }
 
+// A row's vectors: 16-byte ones from the first aligned element, the elements
+// before and after them (under 16 bytes each).  Groups are U vectors, 32 apart,
+// of a chunk of 32 * U.
+template <typename T>
+struct Row {
+    static constexpr int VN = 16 / (int)sizeof(T), N = U * VN;
+    const T *x;
+    const uint4 *v;
+    uint32_t vocab, head, nvec, tail;
+    __device__ __forceinline__ Row(const T *x_, uint32_t vocab_) : x(x_), vocab(vocab_) {
+        head = min(vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
+        nvec = (vocab - head) / VN;
+        tail = vocab - head - nvec * VN;
+        v = reinterpret_cast<const uint4 *>(x + head);
+    }
+    // vectors at + 32 u, -inf past the end
+    __device__ __forceinline__ void load(uint4 (&r)[U], uint32_t at) const {
+        const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = at + 32 * u < nvec ? __ldcs(v + at + 32 * u) : make_uint4(inf, inf, inf, inf);
+    }
+    // two elements of a vector as floats
+    static __device__ __forceinline__ float2 pair(const uint4 &r, int i) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    // the largest element, NaN aside
+    static __device__ __forceinline__ float best(const uint4 (&r)[U]) {
+        if constexpr (sizeof(T) == 4) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(r[u].x), __uint_as_float(r[u].y))),
+                          fmaxf(__uint_as_float(r[u].z), __uint_as_float(r[u].w)));
+            return m;
+        } else {
+            using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+            const T2 *p = reinterpret_cast<const T2 *>(r);
+            T2 m = p[0];
+#pragma unroll
+            for (int i = 1; i < U * 4; ++i) m = __hmax2(m, p[i]);
+            const float a = to_f32(m.x), b = to_f32(m.y);
+            return fmaxf(fmaxf(a, b), -INFINITY);
+        }
+    }
+    __device__ __forceinline__ uint32_t index(uint32_t at, int j) const { return head + (at + 32 * (j / VN)) * VN + j % VN; }
+};
+
+// A descending list with the keys of the lanes in `todo`.  (Not inlined: it is
+// called where few warps go, and its code would be many times the scan's.)
+__device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned todo, int lane) {
+    // sorting and merging cost about as much as 6 single insertions
+    if (__popc(todo) > 6) {
+        key = sort_desc(todo >> lane & 1 ? key : 0, lane);
+        return __any_sync(kAll, list != 0) ? merge_desc(list, key, lane) : key;
+    }
+    while (todo) {
+        const int src = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const uint64_t one = __shfl_sync(kAll, key, src);
+        const int p = __popc(__ballot_sync(kAll, list > one));
+        const uint64_t up = __shfl_up_sync(kAll, list, 1);
+        list = lane < p ? list : lane == p ? one : up;
+    }
+    return list;
+}
+
 // What a warp has seen of its row.
 template <bool TOP>
 struct Warp {
@@ -156,29 +228,14 @@ struct Warp {
         c = c_;
         k = k_;
     }
-    __device__ __forceinline__ void set_thr() {
+    // keys of lanes in `todo` into the list
+    __device__ __forceinline__ void insert(uint64_t key, unsigned todo, int lane) {
+        list = with_keys(list, key, todo, lane);
         kth = __shfl_sync(kAll, list, k - 1);
         const uint32_t o = (uint32_t)(kth >> 32);
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
     }
-    // keys of lanes in `todo` into the list
-    __device__ __forceinline__ void insert(uint64_t key, unsigned todo, int lane) {
-        if (__popc(todo) > 6) {
-            // (sorting and merging cost about as much as 6 single insertions)
-            list = merge_desc(list, sort_desc(todo >> lane & 1 ? key : 0, lane), lane);
-        } else {
-            while (todo) {
-                const int src = __ffs(todo) - 1;
-                todo &= todo - 1;
-                const uint64_t one = __shfl_sync(kAll, key, src);
-                const int p = __popc(__ballot_sync(kAll, list > one));
-                const uint64_t up = __shfl_up_sync(kAll, list, 1);
-                list = lane < p ? list : lane == p ? one : up;
-            }
-        }
-        set_thr();
-    }
-    __device__ __forceinline__ void raise(float best, int lane) {
+    __device__ __forceinline__ void raise(float best) {
         float top = best;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
@@ -199,41 +256,20 @@ struct Warp {
         s2 = add2(s2, e);
         w2 = fma2(e, pack2(fmaxf(u.x, -FLT_MAX), fmaxf(u.y, -FLT_MAX)), w2);
     }
-    // N values a lane, in order of their indices idx(j); those past the row's end
-    // (valid(j) false, the first never before others) are -inf
-    template <int N, typename Idx, typename Valid>
-    __device__ __forceinline__ void take(const float (&x)[N], int lane, const int *shared_thr, Idx idx, Valid valid) {
-        float best = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < N; ++j) best = fmaxf(best, x[j]);
-        // a group can enter the list if it is above the k-th of this warp's, and
-        // not below that of another warp of the CTA
-        bool enters = false;
-        if (TOP) enters = valid(0) && !(best <= thr) && !(shared_thr && best < unordered((uint32_t)*(volatile const int *)shared_thr));
-        if (__any_sync(kAll, enters || best > m)) {
-            raise(best, lane);
-            if constexpr (TOP) {
-                unsigned todo = __ballot_sync(kAll, enters);
-                if (todo) {
-                    uint32_t at = idx(0);
-                    bool any = false;
-#pragma unroll
-                    for (int j = N - 1; j >= 0; --j)
-                        if (x[j] == best && valid(j)) {
-                            at = idx(j);
-                            any = true;
-                        }
-                    const uint64_t key = make_key(any ? best : __uint_as_float(0x7fc00000u), at);
-                    insert(key, todo, lane);
-                }
-            }
+    // A group: `best` its largest element, key() its key, `here` whether the lane
+    // has one.  It can enter the list if it is above the k-th entry, and not below
+    // `floor`, which k groups of the row are known to reach.  True if the list changed.
+    template <typename Key>
+    __device__ __forceinline__ bool offer(float best, bool here, float floor, int lane, Key key) {
+        const bool enters = TOP && here && !(best <= thr) && !(best < floor);
+        if (!__any_sync(kAll, enters || best > m)) return false;
+        raise(best);
+        if constexpr (TOP) {
+            const unsigned todo = __ballot_sync(kAll, enters);
+            if (todo) insert(key(), todo, lane);
+            return todo != 0;
         }
-        if constexpr (N == 1) {
-            add(x[0], -INFINITY);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j += 2) add(x[j], x[j + 1]);
-        }
+        return false;
     }
     // the warp's sums, the same in every lane
     __device__ __forceinline__ Softmax total() const {
@@ -246,38 +282,6 @@ struct Warp {
         }
         return a;
     }
-};
-
-// A row's vectors: 16-byte ones from the first aligned element, the elements
-// before and after them (under 16 bytes each).  Groups are U vectors, 32 apart,
-// of a chunk of 32 * U.
-template <typename T>
-struct Row {
-    static constexpr int VN = 16 / (int)sizeof(T);
-    const T *x;
-    const uint4 *v;
-    uint32_t vocab, head, nvec, tail;
-    __device__ __forceinline__ Row(const T *x_, uint32_t vocab_) : x(x_), vocab(vocab_) {
-        head = min(vocab, (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / (uint32_t)sizeof(T));
-        nvec = (vocab - head) / VN;
-        tail = vocab - head - nvec * VN;
-        v = reinterpret_cast<const uint4 *>(x + head);
-    }
-    // vectors at + 32 u, -inf past the end
-    __device__ __forceinline__ void load(uint4 (&r)[U], uint32_t at) const {
-        const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-#pragma unroll
-        for (int u = 0; u < U; ++u) r[u] = at + 32 * u < nvec ? __ldcs(v + at + 32 * u) : make_uint4(inf, inf, inf, inf);
-    }
-    static __device__ __forceinline__ void unpack(const uint4 (&r)[U], float (&f)[U * VN]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const T *p = reinterpret_cast<const T *>(&r[u]);
-#pragma unroll
-            for (int j = 0; j < VN; ++j) f[u * VN + j] = to_f32(p[j]);
-        }
-    }
-    __device__ __forceinline__ uint32_t index(uint32_t at, int j) const { return head + (at + 32 * (j / VN)) * VN + j % VN; }
 };
 
 struct Args {
@@ -320,16 +324,17 @@ __device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t r
         const uint32_t at = vec / (32 * U) * (32 * U) + vec % 32;
         uint4 raw[U];
         r.load(raw, group ? at : r.nvec);
-        float x[N];
-        Row<T>::unpack(raw, x);
-        st.set_thr();
+        st.insert(0, 0, lane);  // (the k-th of the row)
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const uint32_t idx = r.index(at, j);
-            const uint64_t key = make_key(x[j], idx);
-            const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
-            const unsigned todo = __ballot_sync(kAll, want);
-            if (todo) st.insert(key, todo, lane);
+        for (int j = 0; j < Row<T>::N; ++j) {
+            const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
+            const float x = j & 1 ? p.y : p.x;
+            if (__any_sync(kAll, group && !(x < st.thr))) {
+                const uint64_t key = make_key(x, r.index(at, j));
+                const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
+                const unsigned todo = __ballot_sync(kAll, want);
+                if (todo) st.insert(key, todo, lane);
+            }
         }
         if (lane < g.k) {
             g.top_id[row * g.k + lane] = (int64_t)(uint32_t)~(uint32_t)st.list;
@@ -356,35 +361,67 @@ __device__ __forceinline__ void finish_padding(const Args &g, int64_t row, int l
 
 // Warp `w` of `nw` over one row: chunk i to warp i % nw, the elements outside
 // the vectors to the last warp, one a lane.
+//
+// `reached` (null: none): for each of the CTA's NW warps the value of its best
+// ceil(k / NW)-th group so far.  Their least is reached by k groups of the row,
+// so groups below it cannot be in the answer: the warps' lists together then
+// take in about as many groups as one list over the whole CTA would.
+constexpr int NW = 8;
 template <typename T, bool TOP>
-__device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, int *shared_thr) {
+__device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, uint32_t *reached) {
     const uint32_t step = nw * 32 * U;
     uint32_t v0 = w * 32 * U;
     uint4 next[U];
     if (v0 < r.nvec) r.load(next, v0 + lane);
     while (v0 < r.nvec) {
         const uint32_t at = v0 + lane;
-        float x[U * Row<T>::VN];
-        Row<T>::unpack(next, x);
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = next[u];
         v0 += step;
         if (v0 < r.nvec) r.load(next, v0 + lane);
-        st.take(x, lane, shared_thr, [&](int j) { return r.index(at, j); },
-                [&](int j) { return at + 32 * (j / Row<T>::VN) < r.nvec; });
-        if (TOP && shared_thr && lane == 0 && st.thr == st.thr) atomicMax((unsigned *)shared_thr, ordered(st.thr));
+        float floor = -INFINITY;
+        if (TOP && reached) {
+            const uint32_t o = __reduce_min_sync(kAll, *(volatile uint32_t *)(reached + lane % NW));
+            if (o) floor = unordered(o);
+        }
+        const float best = Row<T>::best(raw);
+        const bool changed = st.offer(best, at < r.nvec, floor, lane, [&] {
+            uint32_t idx = r.index(at, 0);
+            bool any = false;
+#pragma unroll
+            for (int j = Row<T>::N - 1; j >= 0; --j) {
+                const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
+                if ((j & 1 ? p.y : p.x) == best && at + 32 * (j / Row<T>::VN) < r.nvec) {
+                    idx = r.index(at, j);
+                    any = true;
+                }
+            }
+            return make_key(any ? best : __uint_as_float(0x7fc00000u), idx);
+        });
+        if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < Row<T>::VN / 2; ++i) {
+                const float2 p = Row<T>::pair(raw[u], i);
+                st.add(p.x, p.y);
+            }
     }
     if (w == nw - 1 && r.head + r.tail) {
         const bool in = lane < r.head || (lane >= 16 && lane - 16 < r.tail);
         const uint32_t idx = lane < 16 ? lane : r.head + r.nvec * Row<T>::VN + lane - 16;
-        const float x[1] = {in ? to_f32(r.x[idx]) : -INFINITY};
+        const float x = in ? to_f32(r.x[idx]) : -INFINITY;
         // the head's indices are below the list's: equal values enter, too
-        if (TOP && in && x[0] == st.thr) st.thr = __uint_as_float(0x7fc00000u);
-        st.take(x, lane, nullptr, [&](int) { return idx; }, [&](int) { return in; });
+        if (TOP && in && x == st.thr) st.thr = __uint_as_float(0x7fc00000u);
+        st.offer(x, in, -INFINITY, lane, [&] { return make_key(x, idx); });
+        st.add(x, -INFINITY);
     }
 }
 
 // A warp per row
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(256) k_logprobs_warp(const T *__restrict__ x, Args g) {
+__global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ x, Args g) {
     const int lane = threadIdx.x & 31;
     for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < g.rows; row += (int64_t)gridDim.x * 8) {
         if (padding(g, row)) {
@@ -400,17 +437,37 @@ __global__ void __launch_bounds__(256) k_logprobs_warp(const T *__restrict__ x, 
     }
 }
 
-// A cluster of CTAs per row (one CTA without cluster launch): the warps' sums
-// and lists meet in the CTA's shared memory, the CTAs' in the first CTA's warp
-// 0, which reads the others' over distributed shared memory.  No workspace.
+// The CTA's warps' sums and lists, joined in halves into warp 0's: in round h
+// warps under h take those of warps h above.
+template <bool TOP>
+struct Joint {
+    Softmax sums[NW];
+    uint64_t lists[NW][32];
+};
+template <bool TOP>
+__device__ __forceinline__ void join_warps(Joint<TOP> &j, Softmax &a, uint64_t &list, int n, int w, int lane, float c) {
+    for (int h = n >> 1; h > 0; h >>= 1) {
+        if (w >= h && w < 2 * h) {
+            if (lane == 0) j.sums[w] = a;
+            if constexpr (TOP) j.lists[w][lane] = list;
+        }
+        __syncthreads();
+        if (w < h) {
+            join(a, j.sums[w + h], c);
+            if constexpr (TOP) list = merge_desc(list, j.lists[w + h][lane], lane);
+        }
+    }
+}
+
+// A cluster of CTAs per row (1, 2, 4, 8 or 16): the warps' sums and lists meet in
+// the CTA's shared memory, the CTAs' in the first CTA's warps, which read the
+// others' over distributed shared memory.  No workspace.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(256) k_logprobs_cta(const T *__restrict__ x, Args g) {
-    constexpr int NW = 8;
-    __shared__ Softmax sums[NW];
-    __shared__ uint64_t lists[NW][32];
+__global__ void __launch_bounds__(256, LB) k_logprobs_cta(const T *__restrict__ x, Args g) {
+    __shared__ Joint<TOP> joint;
     __shared__ Softmax cta_sums;
     __shared__ uint64_t cta_list[32];
-    __shared__ int thr;
+    __shared__ uint32_t reached[NW];
     auto cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -421,39 +478,37 @@ __global__ void __launch_bounds__(256) k_logprobs_cta(const T *__restrict__ x, A
             continue;
         }
         const Row<T> r(x + row * g.ld, g.vocab);
-        if (threadIdx.x == 0) thr = 0;
-        __syncthreads();
+        if (TOP) {
+            if (threadIdx.x < NW) reached[threadIdx.x] = 0;
+            __syncthreads();
+        }
         Warp<TOP> st;
         st.reset(c, g.k);
-        scan<T, TOP>(st, r, part * NW + w, parts * NW, lane, &thr);
+        scan<T, TOP>(st, r, part * NW + w, parts * NW, lane, reached);
         Softmax a = st.total();
-        if (lane == 0) sums[w] = a;
-        if constexpr (TOP) lists[w][lane] = st.list;
-        __syncthreads();
-        if (w == 0) {
-#pragma unroll
-            for (int i = 1; i < NW; ++i) {
-                join(a, sums[i], c);
-                if constexpr (TOP) st.list = merge_desc(st.list, lists[i][lane], lane);
-            }
-            if (parts > 1) {
+        join_warps<TOP>(joint, a, st.list, NW, w, lane, c);
+        if (parts > 1) {
+            if (w == 0) {
                 if (lane == 0) cta_sums = a;
                 if constexpr (TOP) cta_list[lane] = st.list;
             }
-        }
-        if (parts > 1) {
             cluster.sync();
-            if (part == 0 && w == 0) {
-                for (int i = 1; i < parts; ++i) {
-                    join(a, *cluster.map_shared_rank(&cta_sums, i), c);
-                    if constexpr (TOP) st.list = merge_desc(st.list, cluster.map_shared_rank(cta_list, i)[lane], lane);
+            if (part == 0) {
+                // warp w: CTA w's, and CTA w + 8's
+                if (w > 0 && w < parts) {
+                    a = *cluster.map_shared_rank(&cta_sums, w);
+                    if constexpr (TOP) st.list = cluster.map_shared_rank(cta_list, w)[lane];
                 }
+                if (w + NW < parts) {
+                    join(a, *cluster.map_shared_rank(&cta_sums, w + NW), c);
+                    if constexpr (TOP) st.list = merge_desc(st.list, cluster.map_shared_rank(cta_list, w + NW)[lane], lane);
+                }
+                join_warps<TOP>(joint, a, st.list, min(parts, NW), w, lane, c);
             }
             cluster.sync();  // the others' shared memory is read until here
-        } else {
-            __syncthreads();
         }
         if (part == 0 && w == 0) finish<T, TOP>(g, r, row, a, st, lane);
+        __syncthreads();  // the next row's sums go into the same shared memory
     }
 }
 

@@ -11,12 +11,17 @@
 // element of the block dequantises to NaN.
 //
 // q is the correctly rounded quotient although it comes from an fp32 product
-// p = x * inv, inv = 448 / amax: a point halfway between two e4m3 values has
-// its low 16 bits zero, and p is within two steps of the quotient (half a step
-// from each of its two roundings, at most twice that across a power of two),
-// so p can be on the wrong side only where its low bits are within 2 of zero
-// (one element in 13000).  There the quotient is taken as p + e, with the
-// remainders of both roundings in e.
+// p = x * inv.  A point halfway between two e4m3 values has the low 20 bits
+// 0x80000 (the low 16 zero under 2^-6, where the steps no longer shrink).  A
+// quotient is one of them or, as 448 X = D A has integers on both sides, at
+// least 2^-(5 + bits of A) away from it.
+//   16-bit types: inv is 448 / amax and up to two steps more, so p is the
+//     quotient or up to 4 steps above it in magnitude; with the low 3 bits
+//     cleared a halfway quotient is exact, and any other is 2^-16 away.
+//   float: p is within two steps of the quotient, so it can be on the wrong
+//     side only within two steps of a halfway point (one element in 200000);
+//     there the quotient is taken as p + e, with the remainders of both
+//     roundings in e.
 //
 // Bound by HBM: x is read once (into registers, where it waits for its
 // block's maximum), q and the scales are written once.
@@ -45,21 +50,24 @@ __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[16 / sizeof(T)
     for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = to_f32(p[i]);
 }
 
-// One block's factors: inv = 448 / amax, and what that rounding left, relative.
+// One block's factors: inv (above), and what rounding 448 / amax left, relative.
 struct Factor {
     float inv, rest;
 };
+template <typename T>
 __device__ __forceinline__ Factor factor(float amax) {
     const float inv = __fdiv_rn(kE4M3Max, amax);
+    if (sizeof(T) == 2) return {inv > 0.0f ? __uint_as_float(__float_as_uint(inv) + 2u) : inv, 0.0f};
     return {inv, __fmaf_rn(-amax, inv, kE4M3Max) * (1.0f / kE4M3Max)};
 }
 
-__device__ __forceinline__ bool may_be_halfway(float p) { return ((__float_as_uint(p) + 2u) & 0xffffu) <= 4u; }
+__device__ __forceinline__ bool may_be_halfway(float p) {
+    return ((__float_as_uint(p) - 0x7fffeu) & 0xfffffu) <= 4u || fabsf(p) < 0x1p-6f;
+}
 
 // A float that rounds to the same e4m3 value as 448 x / amax = p + e: the sum,
 // with its last bit set where it is not exact, which no halfway point has.  e
-// is right to 2^-46 of p; a quotient is a halfway point or, as 448 X = D A has
-// integers under 2^33 times powers of two on both sides, 2^-34 away from it.
+// is right to 2^-46 of p, and a quotient that is no halfway point is 2^-34 away.
 __device__ __forceinline__ float quotient(float x, float p, Factor f) {
     const float e = __fmaf_rn(x, f.inv, -p) + p * f.rest;
     const float s = p + e, left = (p - s) + e;
@@ -68,109 +76,199 @@ __device__ __forceinline__ float quotient(float x, float p, Factor f) {
     return !inexact ? s : __uint_as_float((left > 0.0f) == (s > 0.0f) ? b + 1 : b - 1);
 }
 
+// four elements' bytes
+template <typename T>
 __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, Factor f) {
-    float p[4] = {a * f.inv, b * f.inv, c * f.inv, d * f.inv};
-    if (may_be_halfway(p[0]) | may_be_halfway(p[1]) | may_be_halfway(p[2]) | may_be_halfway(p[3])) {
-        // (most often zeros, which stay)
-        if (p[0] != 0.0f && may_be_halfway(p[0])) p[0] = quotient(a, p[0], f);
-        if (p[1] != 0.0f && may_be_halfway(p[1])) p[1] = quotient(b, p[1], f);
-        if (p[2] != 0.0f && may_be_halfway(p[2])) p[2] = quotient(c, p[2], f);
-        if (p[3] != 0.0f && may_be_halfway(p[3])) p[3] = quotient(d, p[3], f);
+    const float x[4] = {a, b, c, d};
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        p[i] = x[i] * f.inv;
+        if (sizeof(T) == 2) p[i] = __uint_as_float(__float_as_uint(p[i]) & ~7u);
+    }
+    if (sizeof(T) == 4 && (may_be_halfway(p[0]) | may_be_halfway(p[1]) | may_be_halfway(p[2]) | may_be_halfway(p[3]))) {
+        // (most often zeros, which stay; under 2^-6 any p takes the longer way)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p[i] != 0.0f) p[i] = quotient(x[i], p[i], f);
     }
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p[0], p[1]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p[2], p[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
 
-// 1 x 128 blocks, 8 lanes to a block and 16 elements to a lane, so that the
-// block's two divisions and the shuffles for its maximum are shared by 16
-// elements (a warp to a block of floats, 4 elements a lane, took 72 us instead
-// of 48 at 32768 x 1536: it was bound by instructions).  VEC: rows of x start
-// on 16 bytes and rows of q on 16 / sizeof(T) bytes, and a lane's elements are
-// 16-byte vectors, 8 vectors apart; otherwise single elements, 8 apart.
-template <typename T, bool VEC, typename I>
+// 1 x 128 blocks where rows of x start on 16 bytes and rows of q on 16 /
+// sizeof(T): 8 lanes to a block and 16 elements to a lane, so that the block's
+// two divisions and the shuffles for its maximum are shared by 16 elements (a
+// warp to a block, 4 elements a lane, was bound by instructions: 72 us instead
+// of 43 at 32768 x 1536 floats).
+template <typename T, typename I>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, I rows, I cols,
                                                        uint8_t *__restrict__ q, int64_t ldq,
                                                        float *__restrict__ scale, int64_t lds) {
-    constexpr int VN = VEC ? 16 / (int)sizeof(T) : 1;  // elements of one access
+    constexpr int VN = 16 / (int)sizeof(T);
     constexpr int LANES = 8, NV = QB / LANES / VN;
+    constexpr int U = 4 / NV;  // blocks of a group of lanes at a time: 64 bytes a thread in flight
     const int lane = threadIdx.x % LANES;
     const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
-    const I first = (I)blockIdx.x * (256 / LANES), step = (I)gridDim.x * (256 / LANES);
-    for (I base = first; base < total; base += step) {
-        const I b = base + (I)(threadIdx.x / LANES);
-        const bool in = b < total;
-        const I row = in ? b / nkb : 0, kb = in ? b - row * nkb : 0;
-        const I c = kb * QB;
-        const int nc = !in ? 0 : cols - c < QB ? (int)(cols - c) : QB;
-        const T *xb = x + (int64_t)row * ldx + c;
-        float v[NV][VN];
+    const I groups = (I)gridDim.x * (256 / LANES);
+    for (I base = (I)blockIdx.x * (256 / LANES); base < total; base += groups * U) {
+        float v[U][NV][VN];
+        I row[U], kb[U];
+        int nc[U];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int at = (lane + LANES * i) * VN;
-            if constexpr (VEC) {
-                if (at + VN <= nc) {
-                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xb + at)), v[i]);
+        for (int u = 0; u < U; ++u) {
+            const I b = base + (I)(threadIdx.x / LANES) + u * groups;
+            const bool in = b < total;
+            row[u] = in ? b / nkb : 0;
+            kb[u] = in ? b - row[u] * nkb : 0;
+            const I c = kb[u] * QB;
+            nc[u] = !in ? 0 : cols - c < QB ? (int)(cols - c) : QB;
+            const T *xb = x + (int64_t)row[u] * ldx + c;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int at = (lane + LANES * i) * VN;
+                if (at + VN <= nc[u]) {
+                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xb + at)), v[u][i]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < VN; ++j) v[i][j] = at + j < nc ? to_f32(xb[at + j]) : 0.0f;
+                    for (int j = 0; j < VN; ++j) v[u][i][j] = at + j < nc[u] ? to_f32(xb[at + j]) : 0.0f;
                 }
-            } else {
-                v[i][0] = at < nc ? to_f32(xb[at]) : 0.0f;
             }
         }
-        float m = kTiny;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int u = 0; u < U; ++u) {
+            float m = kTiny;
 #pragma unroll
-            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[i][j]));
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (!in) continue;
-        const Factor f = factor(m);
-        if (lane == 0) scale[(int64_t)row * lds + kb] = __fdiv_rn(m, kE4M3Max);
-        uint8_t *qb = q + (int64_t)row * ldq + c;
-        if constexpr (VEC) {
+                for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[u][i][j]));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (nc[u] == 0) continue;
+            const Factor f = factor<T>(m);
+            if (lane == 0) scale[(int64_t)row[u] * lds + kb[u]] = __fdiv_rn(m, kE4M3Max);
+            uint8_t *qb = q + (int64_t)row[u] * ldq + kb[u] * QB;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int at = (lane + LANES * i) * VN;
                 uint32_t w[VN / 4];
 #pragma unroll
                 for (int j = 0; j < VN / 4; ++j)
-                    w[j] = quant4(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3], f);
-                if (at + VN <= nc) {
+                    w[j] = quant4<T>(v[u][i][4 * j], v[u][i][4 * j + 1], v[u][i][4 * j + 2], v[u][i][4 * j + 3], f);
+                if (at + VN <= nc[u]) {
                     if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qb + at) = w[0];
                     else *reinterpret_cast<uint2 *>(qb + at) = make_uint2(w[0], w[VN / 4 - 1]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < VN; ++j)
-                        if (at + j < nc) qb[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NV; i += 4) {
-                const uint32_t w = quant4(v[i][0], v[i + 1][0], v[i + 2][0], v[i + 3][0], f);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = lane + LANES * (i + j);
-                    if (at < nc) qb[at] = (uint8_t)(w >> 8 * j);
+                        if (at + j < nc[u]) qb[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
                 }
             }
         }
     }
 }
 
-// 128 x 128 blocks: a CTA of 8 warps per block, which stays in registers (64
+// The same at any alignment: four blocks after one another to a warp, elements
+// 4 lane .. 4 lane + 3 of each to a lane (X4: as one load).  The bytes leave as
+// aligned words, put together from neighbouring lanes' and, within a row,
+// neighbouring blocks': L2 pays for each partly written 32-byte sector (single
+// bytes, 8 to 32 in a row: 66 to 83 us at 11212 x 4229 halves).  Lane i takes the
+// divisions of block i % 4.
+template <typename T, bool X4, typename I>
+__global__ void __launch_bounds__(256) k_quantize_rows_any(const T *__restrict__ x, int64_t ldx, I rows, I cols,
+                                                           uint8_t *__restrict__ q, int64_t ldq,
+                                                           float *__restrict__ scale, int64_t lds) {
+    constexpr int NB = 4;
+    const int lane = threadIdx.x & 31;
+    const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
+    const I step = (I)gridDim.x * (8 * NB);
+    for (I base = ((I)blockIdx.x * 8 + (I)(threadIdx.x >> 5)) * NB; base < total; base += step) {
+        float v[NB][4], m[NB];
+        I row[NB], kb[NB];
+        int nc[NB];
+        row[0] = base / nkb;
+        kb[0] = base - row[0] * nkb;
+#pragma unroll
+        for (int b = 1; b < NB; ++b) {
+            const bool next = kb[b - 1] + 1 == nkb;
+            row[b] = row[b - 1] + (next ? 1 : 0);
+            kb[b] = next ? 0 : kb[b - 1] + 1;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const I left = cols - kb[b] * QB;
+            nc[b] = row[b] >= rows ? 0 : left < QB ? (int)left : QB;
+            const T *xb = x + (int64_t)row[b] * ldx + kb[b] * QB + 4 * lane;
+            if (X4 && 4 * lane + 4 <= nc[b]) {
+                if constexpr (sizeof(T) == 4) {
+                    const float4 f = __ldcs(reinterpret_cast<const float4 *>(xb));
+                    v[b][0] = f.x, v[b][1] = f.y, v[b][2] = f.z, v[b][3] = f.w;
+                } else {
+                    const uint2 f = __ldcs(reinterpret_cast<const uint2 *>(xb));
+                    const T *p = reinterpret_cast<const T *>(&f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[b][j] = to_f32(p[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[b][j] = 4 * lane + j < nc[b] ? to_f32(xb[j]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float a = fmaxf(fmaxf(kTiny, fmaxf(fabsf(v[b][0]), fabsf(v[b][1]))), fmaxf(fabsf(v[b][2]), fabsf(v[b][3])));
+            m[b] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));  // (positive: ordered as its bits)
+        }
+        const int mine = lane % NB;
+        const float mm = mine == 0 ? m[0] : mine == 1 ? m[1] : mine == 2 ? m[2] : m[3];
+        const Factor fm = factor<T>(mm);
+        const float sm = __fdiv_rn(mm, kE4M3Max);
+        uint32_t w[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const Factor f{__shfl_sync(0xffffffffu, fm.inv, b), __shfl_sync(0xffffffffu, fm.rest, b)};
+            w[b] = quant4<T>(v[b][0], v[b][1], v[b][2], v[b][3], f);
+            if (lane == b && nc[b]) scale[(int64_t)row[b] * lds + kb[b]] = sm;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint8_t *qb = q + (int64_t)row[b] * ldq + kb[b] * QB;
+            const int sh = (int)((uintptr_t)qb & 3);
+            // the word that ends before this lane's: the last lane's or the last block's
+            uint32_t before = __shfl_up_sync(0xffffffffu, w[b], 1);
+            const uint32_t last = __shfl_sync(0xffffffffu, w[b > 0 ? b - 1 : 0], 31);
+            const bool linked = b > 0 && row[b > 0 ? b - 1 : 0] == row[b] && nc[b > 0 ? b - 1 : 0] == QB && nc[b] == QB;
+            const bool goes_on = b + 1 < NB && row[b + 1 < NB ? b + 1 : b] == row[b] && nc[b + 1 < NB ? b + 1 : b] == QB;
+            if (lane == 0) before = last;
+            if (nc[b] == QB) {
+                if (lane > 0 || linked || sh == 0) {
+                    *reinterpret_cast<uint32_t *>(qb + 4 * lane - sh) = __funnelshift_l(before, w[b], 8 * sh);
+                } else {
+                    for (int j = 0; j < 4 - sh; ++j) qb[j] = (uint8_t)(w[b] >> 8 * j);
+                }
+                if (lane == 31 && !goes_on)
+                    for (int j = 4 - sh; j < 4; ++j) qb[124 + j] = (uint8_t)(w[b] >> 8 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (4 * lane + j < nc[b]) qb[4 * lane + j] = (uint8_t)(w[b] >> 8 * j);
+            }
+        }
+    }
+}
+
+// 128 x 128 blocks: a CTA of 16 warps per block, which stays in registers (32
 // values a thread) while the maximum crosses the CTA.
+constexpr int kBlockThreads = 512;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int64_t rows,
+__global__ void __launch_bounds__(kBlockThreads, 2) k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int64_t rows,
                                                          int64_t cols, uint8_t *__restrict__ q, int64_t ldq,
                                                          float *__restrict__ scale, int64_t lds) {
     constexpr int VN = VEC ? 16 / (int)sizeof(T) : 4;
-    constexpr int LANES = QB / VN, TALL = 256 / LANES;  // rows per step
+    constexpr int LANES = QB / VN, TALL = kBlockThreads / LANES;  // rows per step
     constexpr int STEPS = QB / TALL;
-    __shared__ float red[8];
+    __shared__ float red[kBlockThreads / 32];
     const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
     const int64_t nkb = (cols + QB - 1) / QB, total = (rows + QB - 1) / QB * nkb;
     for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
@@ -207,9 +305,9 @@ __global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+        for (int w = 0; w < kBlockThreads / 32; ++w) m = fmaxf(m, red[w]);
         __syncthreads();
-        const Factor f = factor(m);
+        const Factor f = factor<T>(m);
         if (threadIdx.x == 0) scale[rb * lds + kb] = __fdiv_rn(m, kE4M3Max);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -219,7 +317,7 @@ __global__ void __launch_bounds__(256) k_quantize_blocks(const T *__restrict__ x
             uint32_t w[VN / 4];
 #pragma unroll
             for (int j = 0; j < VN / 4; ++j)
-                w[j] = quant4(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], f);
+                w[j] = quant4<T>(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], f);
             if constexpr (VEC) {
                 const int at = lane * VN;
                 if (at + VN <= nc) {
@@ -248,25 +346,28 @@ int quantize(lonnx_ctx *ctx, const void *xv, int64_t rows, int64_t cols, int64_t
     const int64_t nkb = (cols + QB - 1) / QB;
     cudaStream_t st = ctx->stream;
     if (block_rows == 1) {
-        const int64_t total = rows * nkb, per_cta = 256 / 8;
+        const int64_t total = rows * nkb, per_cta = 256 / 8;  // (both kernels: 32 blocks a CTA)
         const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, (int64_t)ctx->num_sms * 32);
         // 32-bit indices (one 32-bit division per block) where blocks and columns allow it
-        const bool small = total + (int64_t)grid * per_cta < (1ll << 31) && cols < (1ll << 30);
+        const bool small = total + (int64_t)grid * per_cta * 2 < (1ll << 31) && cols < (1ll << 30);
+        const bool x4 = ((uintptr_t)x & (4 * sizeof(T) - 1)) == 0 && ldx % 4 == 0;
         if (vec && small)
-            k_quantize_rows<T, true, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
+            k_quantize_rows<T, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
         else if (vec)
-            k_quantize_rows<T, true, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+            k_quantize_rows<T, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        else if (small && x4)
+            k_quantize_rows_any<T, true, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
         else if (small)
-            k_quantize_rows<T, false, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
+            k_quantize_rows_any<T, false, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
         else
-            k_quantize_rows<T, false, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+            k_quantize_rows_any<T, false, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
     } else {
         const int64_t total = (rows + QB - 1) / QB * nkb;
         const unsigned grid = (unsigned)std::min<int64_t>(total, 1ll << 30);
         if (vec)
-            k_quantize_blocks<T, true><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+            k_quantize_blocks<T, true><<<grid, kBlockThreads, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
         else
-            k_quantize_blocks<T, false><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+            k_quantize_blocks<T, false><<<grid, kBlockThreads, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
     }
     LONNX_CHECK_LAUNCH(ctx);
     return LONNX_OK;
