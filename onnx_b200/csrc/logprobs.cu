@@ -17,7 +17,9 @@
 // its key is its best element under (value, lowest index first).  The k best
 // elements lie in the k groups of the best keys, so the scan lists groups, with
 // one comparison per 64 bytes and lane, and the elements of the k listed groups
-// are read again at the end.  (A list of elements took a comparison each and
+// are read again at the end.  A key holds the group's first index instead of its
+// best element's unless two groups of a chunk enter with the same value: chunks
+// are runs of the row, so between chunks either index gives the same order.  (A list of elements took a comparison each and
 // four times the insertions: at one row of 250037 floats and k = 20 it made
 // the kernel 32 us instead of 10.)
 //
@@ -37,9 +39,6 @@
 
 namespace cg = cooperative_groups;
 
-#ifndef LB
-#define LB 3
-#endif
 namespace {
 
 constexpr int kMaxTop = 32;  // one list entry per lane
@@ -189,6 +188,20 @@ struct Row {
         }
     }
     __device__ __forceinline__ uint32_t index(uint32_t at, int j) const { return head + (at + 32 * (j / VN)) * VN + j % VN; }
+    // the best element's key (a NaN's where there is nothing else)
+    __device__ __forceinline__ uint64_t best_key(const uint4 (&r)[U], float best, uint32_t at) const {
+        uint32_t idx = index(at, 0);
+        bool any = false;
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) {
+            const float2 p = pair(r[j / VN], j % VN / 2);
+            if ((j & 1 ? p.y : p.x) == best && at + 32 * (j / VN) < nvec) {
+                idx = index(at, j);
+                any = true;
+            }
+        }
+        return make_key(any ? best : __uint_as_float(0x7fc00000u), idx);
+    }
 };
 
 // A descending list with the keys of the lanes in `todo`.  (Not inlined: it is
@@ -236,10 +249,7 @@ struct Warp {
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
     }
     __device__ __forceinline__ void raise(float best) {
-        float top = best;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-        if (!(top > m)) return;
+        const float top = unordered(__reduce_max_sync(kAll, ordered(best)));
         const float2 s = unpack2(s2), w = unpack2(w2);
         Softmax a{m, s.x, w.x}, b{m, s.y, w.y};
         rescale(a, top, c);
@@ -256,17 +266,27 @@ struct Warp {
         s2 = add2(s2, e);
         w2 = fma2(e, pack2(fmaxf(u.x, -FLT_MAX), fmaxf(u.y, -FLT_MAX)), w2);
     }
-    // A group: `best` its largest element, key() its key, `here` whether the lane
-    // has one.  It can enter the list if it is above the k-th entry, and not below
-    // `floor`, which k groups of the row are known to reach.  True if the list changed.
+    // A group: `best` its largest element, first its first index, exact() its best
+    // element's key, `here` whether the lane has one.  It can enter the list if it
+    // is above the k-th entry, and not below `floor`, which k groups of the row are
+    // known to reach.  True if the list changed.
     template <typename Key>
-    __device__ __forceinline__ bool offer(float best, bool here, float floor, int lane, Key key) {
-        const bool enters = TOP && here && !(best <= thr) && !(best < floor);
-        if (!__any_sync(kAll, enters || best > m)) return false;
-        raise(best);
+    __device__ __forceinline__ bool offer(float best, bool here, float floor, int lane, uint32_t first, Key exact) {
+        const bool enters = TOP && here && !(best <= thr) && !(best < floor), higher = best > m;
+        if (!__any_sync(kAll, enters || higher)) return false;
+        if (__any_sync(kAll, higher)) raise(best);
         if constexpr (TOP) {
             const unsigned todo = __ballot_sync(kAll, enters);
-            if (todo) insert(key(), todo, lane);
+            if (todo) {
+                // (-inf: the group may have nothing but NaN)
+                bool alike = false;
+                if (enters) {  // (every lane of `todo` takes part in the match)
+                    const unsigned same = __match_any_sync(todo, best + 0.0f);
+                    alike = same != 1u << lane || best == -INFINITY;
+                }
+                const uint64_t key = __any_sync(kAll, alike) ? exact() : make_key(best, first);
+                insert(key, todo, lane);
+            }
             return todo != 0;
         }
         return false;
@@ -317,20 +337,23 @@ __device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t r
         if (g.entropy) g.entropy[row] = none ? 0.0f : fmaf(a.w / a.s, -0.69314718055994530942f, log_s);
     }
     if constexpr (TOP) {
-        // the listed groups' other elements; an element outside the vectors is a group of its own
-        const uint64_t mine = st.list;
-        const uint32_t i = ~(uint32_t)mine - r.head, vec = i / Row<T>::VN;
-        const bool group = lane < g.k && mine && ~(uint32_t)mine >= r.head && vec < r.nvec;
+        // the listed groups' elements, best ones first; an element outside the
+        // vectors is a group of its own
+        const uint32_t i = ~(uint32_t)st.list - r.head, vec = i / Row<T>::VN;
+        const bool group = lane < g.k && st.list && ~(uint32_t)st.list >= r.head && vec < r.nvec;
         const uint32_t at = vec / (32 * U) * (32 * U) + vec % 32;
         uint4 raw[U];
         r.load(raw, group ? at : r.nvec);
-        st.insert(0, 0, lane);  // (the k-th of the row)
+        const uint64_t mine = group ? r.best_key(raw, Row<T>::best(raw), at) : lane < g.k ? st.list : 0;
+        st.list = 0;
+        st.insert(mine, kAll, lane);
 #pragma unroll
-        for (int j = 0; j < Row<T>::N; ++j) {
+        for (int j = 0; j < Row<T>::N; j += 2) {
             const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
-            const float x = j & 1 ? p.y : p.x;
-            if (__any_sync(kAll, group && !(x < st.thr))) {
-                const uint64_t key = make_key(x, r.index(at, j));
+            if (!__any_sync(kAll, group && !(p.x < st.thr && p.y < st.thr))) continue;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint64_t key = make_key(e ? p.y : p.x, r.index(at, j + e));
                 const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
                 const unsigned todo = __ballot_sync(kAll, want);
                 if (todo) st.insert(key, todo, lane);
@@ -386,19 +409,7 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
             if (o) floor = unordered(o);
         }
         const float best = Row<T>::best(raw);
-        const bool changed = st.offer(best, at < r.nvec, floor, lane, [&] {
-            uint32_t idx = r.index(at, 0);
-            bool any = false;
-#pragma unroll
-            for (int j = Row<T>::N - 1; j >= 0; --j) {
-                const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
-                if ((j & 1 ? p.y : p.x) == best && at + 32 * (j / Row<T>::VN) < r.nvec) {
-                    idx = r.index(at, j);
-                    any = true;
-                }
-            }
-            return make_key(any ? best : __uint_as_float(0x7fc00000u), idx);
-        });
+        const bool changed = st.offer(best, at < r.nvec, floor, lane, r.index(at, 0), [&] { return r.best_key(raw, best, at); });
         if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -414,7 +425,7 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
         const float x = in ? to_f32(r.x[idx]) : -INFINITY;
         // the head's indices are below the list's: equal values enter, too
         if (TOP && in && x == st.thr) st.thr = __uint_as_float(0x7fc00000u);
-        st.offer(x, in, -INFINITY, lane, [&] { return make_key(x, idx); });
+        st.offer(x, in, -INFINITY, lane, idx, [&] { return make_key(x, idx); });
         st.add(x, -INFINITY);
     }
 }
@@ -463,7 +474,7 @@ __device__ __forceinline__ void join_warps(Joint<TOP> &j, Softmax &a, uint64_t &
 // the CTA's shared memory, the CTAs' in the first CTA's warps, which read the
 // others' over distributed shared memory.  No workspace.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(256, LB) k_logprobs_cta(const T *__restrict__ x, Args g) {
+__global__ void __launch_bounds__(256, TOP ? 4 : 3) k_logprobs_cta(const T *__restrict__ x, Args g) {
     __shared__ Joint<TOP> joint;
     __shared__ Softmax cta_sums;
     __shared__ uint64_t cta_list[32];

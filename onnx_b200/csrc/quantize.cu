@@ -101,68 +101,95 @@ __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, F
 // sizeof(T): 8 lanes to a block and 16 elements to a lane, so that the block's
 // two divisions and the shuffles for its maximum are shared by 16 elements (a
 // warp to a block, 4 elements a lane, was bound by instructions: 72 us instead
-// of 43 at 32768 x 1536 floats).
+// of 43 at 32768 x 1536 floats).  The next 64 bytes a thread are in flight
+// meanwhile.
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, I rows, I cols,
                                                        uint8_t *__restrict__ q, int64_t ldq,
                                                        float *__restrict__ scale, int64_t lds) {
     constexpr int VN = 16 / (int)sizeof(T);
     constexpr int LANES = 8, NV = QB / LANES / VN;
-    constexpr int U = 4 / NV;  // blocks of a group of lanes at a time: 64 bytes a thread in flight
+    constexpr int U = 4 / NV;  // blocks of a group of lanes at a time: 64 bytes a thread
     const int lane = threadIdx.x % LANES;
-    const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
-    const I groups = (I)gridDim.x * (256 / LANES);
-    for (I base = (I)blockIdx.x * (256 / LANES); base < total; base += groups * U) {
-        float v[U][NV][VN];
-        I row[U], kb[U];
-        int nc[U];
+    const I nkb = (cols + QB - 1) / QB;
+    const I groups = (I)gridDim.x * (256 / LANES), srow = groups / nkb, skb = groups - srow * nkb;
+    I b0 = (I)blockIdx.x * (256 / LANES) + (I)(threadIdx.x / LANES), row = b0 / nkb, kb = b0 - row * nkb;
+    const auto advance = [&] {  // to the block `groups` further on
+        row += srow;
+        kb += skb;
+        if (kb >= nkb) kb -= nkb, ++row;
+    };
+    const auto fetch = [&](uint4 (&raw)[NV], I row_, I kb_) {  // elements past the row's end are 0
+        const T *xb = x + (int64_t)row_ * ldx + kb_ * QB;
+        const int nc = row_ >= rows ? 0 : cols - kb_ * QB < QB ? (int)(cols - kb_ * QB) : QB;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const I b = base + (I)(threadIdx.x / LANES) + u * groups;
-            const bool in = b < total;
-            row[u] = in ? b / nkb : 0;
-            kb[u] = in ? b - row[u] * nkb : 0;
-            const I c = kb[u] * QB;
-            nc[u] = !in ? 0 : cols - c < QB ? (int)(cols - c) : QB;
-            const T *xb = x + (int64_t)row[u] * ldx + c;
+        for (int i = 0; i < NV; ++i) {
+            const int at = (lane + LANES * i) * VN;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (at + VN <= nc) {
+                raw[i] = __ldcs(reinterpret_cast<const uint4 *>(xb + at));
+            } else if (at < nc) {
+                T part[VN];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int at = (lane + LANES * i) * VN;
-                if (at + VN <= nc[u]) {
-                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xb + at)), v[u][i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VN; ++j) v[u][i][j] = at + j < nc[u] ? to_f32(xb[at + j]) : 0.0f;
-                }
+                for (int j = 0; j < VN; ++j) part[j] = at + j < nc ? xb[at + j] : T(0.0f);
+                raw[i] = *reinterpret_cast<const uint4 *>(part);
             }
         }
+    };
+    uint4 next[U][NV];
+    I nrow[U], nkbs[U];
+    const auto fetch_all = [&] {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            nrow[u] = row, nkbs[u] = kb;
+            fetch(next[u], row, kb);
+            advance();
+        }
+    };
+    fetch_all();
+    // (a warp's four groups of lanes have neighbouring blocks: it ends with the last)
+    while (__any_sync(0xffffffffu, nrow[0] < rows)) {
+        uint4 raw[U][NV];
+        I r[U], k[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            r[u] = nrow[u], k[u] = nkbs[u];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[u][i] = next[u][i];
+        }
+        fetch_all();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float m = kTiny;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                float v[VN];
+                unpack<T>(raw[u][i], v);
 #pragma unroll
-                for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[u][i][j]));
+                for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[j]));
+            }
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (nc[u] == 0) continue;
+            if (r[u] >= rows) continue;
+            const int nc = cols - k[u] * QB < QB ? (int)(cols - k[u] * QB) : QB;
             const Factor f = factor<T>(m);
-            if (lane == 0) scale[(int64_t)row[u] * lds + kb[u]] = __fdiv_rn(m, kE4M3Max);
-            uint8_t *qb = q + (int64_t)row[u] * ldq + kb[u] * QB;
+            if (lane == 0) scale[(int64_t)r[u] * lds + k[u]] = __fdiv_rn(m, kE4M3Max);
+            uint8_t *qb = q + (int64_t)r[u] * ldq + k[u] * QB;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int at = (lane + LANES * i) * VN;
+                float v[VN];
+                unpack<T>(raw[u][i], v);
                 uint32_t w[VN / 4];
 #pragma unroll
-                for (int j = 0; j < VN / 4; ++j)
-                    w[j] = quant4<T>(v[u][i][4 * j], v[u][i][4 * j + 1], v[u][i][4 * j + 2], v[u][i][4 * j + 3], f);
-                if (at + VN <= nc[u]) {
+                for (int j = 0; j < VN / 4; ++j) w[j] = quant4<T>(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], f);
+                if (at + VN <= nc) {
                     if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qb + at) = w[0];
                     else *reinterpret_cast<uint2 *>(qb + at) = make_uint2(w[0], w[VN / 4 - 1]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < VN; ++j)
-                        if (at + j < nc[u]) qb[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+                        if (at + j < nc) qb[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
                 }
             }
         }
