@@ -266,6 +266,16 @@ struct Warp {
         s2 = add2(s2, e);
         w2 = fma2(e, pack2(fmaxf(u.x, -FLT_MAX), fmaxf(u.y, -FLT_MAX)), w2);
     }
+    template <typename T>
+    __device__ __forceinline__ void sum(const Row<T> &, const uint4 (&raw)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < Row<T>::VN / 2; ++i) {
+                const float2 p = Row<T>::pair(raw[u], i);
+                add(p.x, p.y);
+            }
+    }
     // A group: `best` its largest element, first its first index, exact() its best
     // element's key, `here` whether the lane has one.  It can enter the list if it
     // is above the k-th entry, and not below `floor`, which k groups of the row are
@@ -316,12 +326,43 @@ struct Args {
     int *flags;
 };
 
-// The row's answer from its sums and list of groups: one warp, every lane with
+// The list of groups to one of elements: lanes with `group` hold theirs in `raw`
+// (vectors at + 32 u), others the key of a group of one element or 0 in `single`.
+template <typename T>
+__device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, const uint4 (&raw)[U], uint32_t at,
+                                              bool group, uint64_t single, int lane) {
+    const uint64_t mine = group ? r.best_key(raw, Row<T>::best(raw), at) : single;
+    st.list = 0;
+    st.insert(mine, kAll, lane);  // the best of each group first
+#pragma unroll
+    for (int j = 0; j < Row<T>::N; j += 2) {
+        const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
+        if (!__any_sync(kAll, group && !(p.x < st.thr && p.y < st.thr))) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint64_t key = make_key(e ? p.y : p.x, r.index(at, j + e));
+            const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
+            const unsigned todo = __ballot_sync(kAll, want);
+            if (todo) st.insert(key, todo, lane);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, int lane) {
+    // an element outside the vectors is a group of its own
+    const uint32_t i = ~(uint32_t)st.list - r.head, vec = i / Row<T>::VN;
+    const bool in = lane < st.k && st.list, group = in && ~(uint32_t)st.list >= r.head && vec < r.nvec;
+    const uint32_t at = vec / (32 * U) * (32 * U) + vec % 32;
+    uint4 raw[U];
+    r.load(raw, group ? at : r.nvec);
+    list_elements(st, r, raw, at, group, in ? st.list : 0, lane);
+}
+
+// The row's answer from its sums and list of elements: one warp, every lane with
 // the same `a`.
 template <typename T, bool TOP>
-__device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t row, const Softmax &a, Warp<TOP> &st,
+__device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t row, const Softmax &a, const Warp<TOP> &st,
                                        int lane) {
-    constexpr int N = U * Row<T>::VN;
     const bool none = a.s == 0.0f;  // every logit -inf: no token has any probability
     const float log_s = logf(a.s);
     if (lane == 0) {
@@ -337,28 +378,6 @@ __device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t r
         if (g.entropy) g.entropy[row] = none ? 0.0f : fmaf(a.w / a.s, -0.69314718055994530942f, log_s);
     }
     if constexpr (TOP) {
-        // the listed groups' elements, best ones first; an element outside the
-        // vectors is a group of its own
-        const uint32_t i = ~(uint32_t)st.list - r.head, vec = i / Row<T>::VN;
-        const bool group = lane < g.k && st.list && ~(uint32_t)st.list >= r.head && vec < r.nvec;
-        const uint32_t at = vec / (32 * U) * (32 * U) + vec % 32;
-        uint4 raw[U];
-        r.load(raw, group ? at : r.nvec);
-        const uint64_t mine = group ? r.best_key(raw, Row<T>::best(raw), at) : lane < g.k ? st.list : 0;
-        st.list = 0;
-        st.insert(mine, kAll, lane);
-#pragma unroll
-        for (int j = 0; j < Row<T>::N; j += 2) {
-            const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
-            if (!__any_sync(kAll, group && !(p.x < st.thr && p.y < st.thr))) continue;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint64_t key = make_key(e ? p.y : p.x, r.index(at, j + e));
-                const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
-                const unsigned todo = __ballot_sync(kAll, want);
-                if (todo) st.insert(key, todo, lane);
-            }
-        }
         if (lane < g.k) {
             g.top_id[row * g.k + lane] = (int64_t)(uint32_t)~(uint32_t)st.list;
             g.top_logprob[row * g.k + lane] =
@@ -382,15 +401,27 @@ __device__ __forceinline__ void finish_padding(const Args &g, int64_t row, int l
         }
 }
 
+// the elements outside the vectors, one a lane
+template <typename T, bool TOP>
+__device__ __forceinline__ void edges(Warp<TOP> &st, const Row<T> &r, int lane) {
+    if (r.head + r.tail == 0) return;
+    const bool in = lane < r.head || (lane >= 16 && lane - 16 < r.tail);
+    const uint32_t idx = lane < 16 ? lane : r.head + r.nvec * Row<T>::VN + lane - 16;
+    const float x = in ? to_f32(r.x[idx]) : -INFINITY;
+    // the head's indices are below the list's: equal values enter, too
+    if (TOP && in && x == st.thr) st.thr = __uint_as_float(0x7fc00000u);
+    st.offer(x, in, -INFINITY, lane, idx, [&] { return make_key(x, idx); });
+    st.add(x, -INFINITY);
+}
+
 // Warp `w` of `nw` over one row: chunk i to warp i % nw, the elements outside
-// the vectors to the last warp, one a lane.
+// the vectors to the last warp.
 //
 // `reached` (null: none): for each of the CTA's NW warps the value of its best
 // ceil(k / NW)-th group so far.  Their least is reached by k groups of the row,
 // so groups below it cannot be in the answer: the warps' lists together then
 // take in about as many groups as one list over the whole CTA would.
-constexpr int NW = 8;
-template <typename T, bool TOP>
+template <int NW, typename T, bool TOP>
 __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, uint32_t *reached) {
     const uint32_t step = nw * 32 * U;
     uint32_t v0 = w * 32 * U;
@@ -411,23 +442,9 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
         const float best = Row<T>::best(raw);
         const bool changed = st.offer(best, at < r.nvec, floor, lane, r.index(at, 0), [&] { return r.best_key(raw, best, at); });
         if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < Row<T>::VN / 2; ++i) {
-                const float2 p = Row<T>::pair(raw[u], i);
-                st.add(p.x, p.y);
-            }
+        st.sum(r, raw);
     }
-    if (w == nw - 1 && r.head + r.tail) {
-        const bool in = lane < r.head || (lane >= 16 && lane - 16 < r.tail);
-        const uint32_t idx = lane < 16 ? lane : r.head + r.nvec * Row<T>::VN + lane - 16;
-        const float x = in ? to_f32(r.x[idx]) : -INFINITY;
-        // the head's indices are below the list's: equal values enter, too
-        if (TOP && in && x == st.thr) st.thr = __uint_as_float(0x7fc00000u);
-        st.offer(x, in, -INFINITY, lane, idx, [&] { return make_key(x, idx); });
-        st.add(x, -INFINITY);
-    }
+    if (w == nw - 1) edges(st, r, lane);
 }
 
 // A warp per row
@@ -443,20 +460,34 @@ __global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ 
         const float c = g.inv_t * 1.44269504088896340736f;
         Warp<TOP> st;
         st.reset(c, g.k);
-        scan<T, TOP>(st, r, 0, 1, lane, nullptr);
+        if (TOP && r.nvec <= 32 * U) {
+            // one chunk: its groups are here, so the list is of elements at once
+            if constexpr (TOP) {
+                uint4 raw[U];
+                r.load(raw, lane);
+                const float best = Row<T>::best(raw);
+                if (__any_sync(kAll, best > st.m)) st.raise(best);
+                list_elements(st, r, raw, lane, lane < r.nvec, 0, lane);
+                st.sum(r, raw);
+                edges(st, r, lane);
+            }
+        } else {
+            scan<1, T, TOP>(st, r, 0, 1, lane, nullptr);
+            if constexpr (TOP) list_elements(st, r, lane);
+        }
         finish<T, TOP>(g, r, row, st.total(), st, lane);
     }
 }
 
 // The CTA's warps' sums and lists, joined in halves into warp 0's: in round h
 // warps under h take those of warps h above.
-template <bool TOP>
+template <int NW>
 struct Joint {
     Softmax sums[NW];
     uint64_t lists[NW][32];
 };
-template <bool TOP>
-__device__ __forceinline__ void join_warps(Joint<TOP> &j, Softmax &a, uint64_t &list, int n, int w, int lane, float c) {
+template <int NW, bool TOP>
+__device__ __forceinline__ void join_warps(Joint<NW> &j, Softmax &a, uint64_t &list, int n, int w, int lane, float c) {
     for (int h = n >> 1; h > 0; h >>= 1) {
         if (w >= h && w < 2 * h) {
             if (lane == 0) j.sums[w] = a;
@@ -473,9 +504,9 @@ __device__ __forceinline__ void join_warps(Joint<TOP> &j, Softmax &a, uint64_t &
 // A cluster of CTAs per row (1, 2, 4, 8 or 16): the warps' sums and lists meet in
 // the CTA's shared memory, the CTAs' in the first CTA's warps, which read the
 // others' over distributed shared memory.  No workspace.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(256, TOP ? 4 : 3) k_logprobs_cta(const T *__restrict__ x, Args g) {
-    __shared__ Joint<TOP> joint;
+template <int NW, typename T, bool TOP>
+__global__ void __launch_bounds__(32 * NW, (TOP ? 32 : 24) / NW) k_logprobs_cta(const T *__restrict__ x, Args g) {
+    __shared__ Joint<NW> joint;
     __shared__ Softmax cta_sums;
     __shared__ uint64_t cta_list[32];
     __shared__ uint32_t reached[NW];
@@ -495,9 +526,9 @@ __global__ void __launch_bounds__(256, TOP ? 4 : 3) k_logprobs_cta(const T *__re
         }
         Warp<TOP> st;
         st.reset(c, g.k);
-        scan<T, TOP>(st, r, part * NW + w, parts * NW, lane, reached);
+        scan<NW, T, TOP>(st, r, part * NW + w, parts * NW, lane, reached);
         Softmax a = st.total();
-        join_warps<TOP>(joint, a, st.list, NW, w, lane, c);
+        join_warps<NW, TOP>(joint, a, st.list, NW, w, lane, c);
         if (parts > 1) {
             if (w == 0) {
                 if (lane == 0) cta_sums = a;
@@ -505,42 +536,34 @@ __global__ void __launch_bounds__(256, TOP ? 4 : 3) k_logprobs_cta(const T *__re
             }
             cluster.sync();
             if (part == 0) {
-                // warp w: CTA w's, and CTA w + 8's
+                // warp w: CTAs w, w + NW, ..
                 if (w > 0 && w < parts) {
                     a = *cluster.map_shared_rank(&cta_sums, w);
                     if constexpr (TOP) st.list = cluster.map_shared_rank(cta_list, w)[lane];
                 }
-                if (w + NW < parts) {
-                    join(a, *cluster.map_shared_rank(&cta_sums, w + NW), c);
-                    if constexpr (TOP) st.list = merge_desc(st.list, cluster.map_shared_rank(cta_list, w + NW)[lane], lane);
+                for (int i = w + NW; i < parts; i += NW) {
+                    join(a, *cluster.map_shared_rank(&cta_sums, i), c);
+                    if constexpr (TOP) st.list = merge_desc(st.list, cluster.map_shared_rank(cta_list, i)[lane], lane);
                 }
-                join_warps<TOP>(joint, a, st.list, min(parts, NW), w, lane, c);
             }
-            cluster.sync();  // the others' shared memory is read until here
+            cluster.barrier_arrive();  // the others' shared memory is read until here
+            if (part == 0) join_warps<NW, TOP>(joint, a, st.list, min(parts, NW), w, lane, c);
         }
-        if (part == 0 && w == 0) finish<T, TOP>(g, r, row, a, st, lane);
+        if (part == 0 && w == 0) {
+            if constexpr (TOP) list_elements(st, r, lane);
+            finish<T, TOP>(g, r, row, a, st, lane);
+        }
+        if (parts > 1) cluster.barrier_wait();
         __syncthreads();  // the next row's sums go into the same shared memory
     }
 }
 
-template <typename T, bool TOP>
-int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
-    const T *x = static_cast<const T *>(xv);
-    const int64_t row_bytes = (int64_t)g.vocab * (int)sizeof(T);
-    // Up to one chunk's worth a warp of a CTA, a warp has a row of its own.
-    if (row_bytes <= 8192) {
-        const unsigned grid = (unsigned)std::min<int64_t>((g.rows + 7) / 8, 1 << 30);
-        k_logprobs_warp<T, TOP><<<grid, 256, 0, ctx->stream>>>(x, g);
-        LONNX_CHECK_LAUNCH(ctx);
-        return LONNX_OK;
-    }
-    // Few rows: as many CTAs to a row as fill the SMs twice, while each still has 16 KB to read.
-    int parts = 1;
-    while (parts < 16 && g.rows * parts < 2 * ctx->num_sms && row_bytes / (parts * 2) >= 16384) parts *= 2;
-    auto kernel = k_logprobs_cta<T, TOP>;
+template <int NW, typename T, bool TOP>
+int launch_cta(lonnx_ctx *ctx, const T *x, const Args &g, int parts) {
+    auto kernel = k_logprobs_cta<NW, T, TOP>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min<int64_t>(g.rows, (1 << 30) / parts) * parts));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(32 * NW);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -556,6 +579,27 @@ int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
     ctx->launches++;
     LONNX_CUDA(cudaLaunchKernelEx(&cfg, kernel, x, g));
     return LONNX_OK;
+}
+
+template <typename T, bool TOP>
+int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
+    const T *x = static_cast<const T *>(xv);
+    const int64_t row_bytes = (int64_t)g.vocab * (int)sizeof(T);
+    // A warp to a row for short rows, or for enough of them to fill the SMs with
+    // warps (5000 x 20000 bfloat16, 5 alternatives: 73 us, 4 warps to a row 95, 8
+    // warps 127); 4 warps, as joining their lists leaves fewer idle, while SMs get
+    // 4 rows each (1000 x 10000: 19 us, 8 warps 25; 300 x 50000: 24 us, 8 warps 23).
+    if (row_bytes <= 8192 || g.rows >= 24 * ctx->num_sms) {
+        const unsigned grid = (unsigned)std::min<int64_t>((g.rows + 7) / 8, 1 << 30);
+        k_logprobs_warp<T, TOP><<<grid, 256, 0, ctx->stream>>>(x, g);
+        LONNX_CHECK_LAUNCH(ctx);
+        return LONNX_OK;
+    }
+    if (TOP && g.rows >= 4 * ctx->num_sms) return launch_cta<4, T, TOP>(ctx, x, g, 1);
+    // Few rows: as many CTAs to a row as fill the SMs twice, while each still has 16 KB to read.
+    int parts = 1;
+    while (parts < 16 && g.rows * parts < 2 * ctx->num_sms && row_bytes / (parts * 2) >= 16384) parts *= 2;
+    return launch_cta<8, T, TOP>(ctx, x, g, parts);
 }
 
 template <typename T>

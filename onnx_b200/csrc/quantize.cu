@@ -196,50 +196,44 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, 
     }
 }
 
-// The same at any alignment: four blocks after one another to a warp, elements
-// 4 lane .. 4 lane + 3 of each to a lane (X4: as one load).  The bytes leave as
-// aligned words, put together from neighbouring lanes' and, within a row,
-// neighbouring blocks': L2 pays for each partly written 32-byte sector (single
-// bytes, 8 to 32 in a row: 66 to 83 us at 11212 x 4229 halves).  Lane i takes the
-// divisions of block i % 4.
-template <typename T, bool X4, typename I>
-__global__ void __launch_bounds__(256) k_quantize_rows_any(const T *__restrict__ x, int64_t ldx, I rows, I cols,
-                                                           uint8_t *__restrict__ q, int64_t ldq,
-                                                           float *__restrict__ scale, int64_t lds) {
-    constexpr int NB = 4;
+// The same at any alignment: a run of up to four blocks of a row to a warp,
+// elements 4 lane .. 4 lane + 3 of each block to a lane (X4: as one load).  The
+// bytes leave as aligned words, put together from neighbouring lanes' and
+// blocks': L2 pays for each partly written 32-byte sector (single bytes, 8 to 32
+// in a row: 66 to 83 us at 11212 x 4229 halves).  Lane b takes the divisions of
+// block b.
+template <typename T, bool X4>
+__global__ void __launch_bounds__(256, 4) k_quantize_rows_any(const T *__restrict__ x, int64_t ldx, int64_t rows,
+                                                              int64_t cols, uint8_t *__restrict__ q, int64_t ldq,
+                                                              float *__restrict__ scale, int64_t lds) {
+    constexpr int NB = 4, RUN = NB * QB;
     const int lane = threadIdx.x & 31;
-    const I nkb = (cols + QB - 1) / QB, total = rows * nkb;
-    const I step = (I)gridDim.x * (8 * NB);
-    for (I base = ((I)blockIdx.x * 8 + (I)(threadIdx.x >> 5)) * NB; base < total; base += step) {
+    const int64_t runs = (cols + RUN - 1) / RUN, warps = (int64_t)gridDim.x * 8;
+    const int64_t srow = warps / runs, srun = warps - srow * runs;
+    const int64_t first = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    int64_t row = first / runs, run = first - row * runs;
+    while (row < rows) {
+        const T *xb = x + row * ldx + run * RUN + 4 * lane;
+        uint8_t *qb = q + row * ldq + run * RUN;
+        float *sb = scale + row * lds + run * NB;
+        const int nc = (int)min((int64_t)RUN, cols - run * RUN);  // columns of the run
         float v[NB][4], m[NB];
-        I row[NB], kb[NB];
-        int nc[NB];
-        row[0] = base / nkb;
-        kb[0] = base - row[0] * nkb;
-#pragma unroll
-        for (int b = 1; b < NB; ++b) {
-            const bool next = kb[b - 1] + 1 == nkb;
-            row[b] = row[b - 1] + (next ? 1 : 0);
-            kb[b] = next ? 0 : kb[b - 1] + 1;
-        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const I left = cols - kb[b] * QB;
-            nc[b] = row[b] >= rows ? 0 : left < QB ? (int)left : QB;
-            const T *xb = x + (int64_t)row[b] * ldx + kb[b] * QB + 4 * lane;
-            if (X4 && 4 * lane + 4 <= nc[b]) {
+            const int at = b * QB + 4 * lane;
+            if (X4 && at + 4 <= nc) {
                 if constexpr (sizeof(T) == 4) {
-                    const float4 f = __ldcs(reinterpret_cast<const float4 *>(xb));
+                    const float4 f = __ldcs(reinterpret_cast<const float4 *>(xb + b * QB));
                     v[b][0] = f.x, v[b][1] = f.y, v[b][2] = f.z, v[b][3] = f.w;
                 } else {
-                    const uint2 f = __ldcs(reinterpret_cast<const uint2 *>(xb));
+                    const uint2 f = __ldcs(reinterpret_cast<const uint2 *>(xb + b * QB));
                     const T *p = reinterpret_cast<const T *>(&f);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[b][j] = to_f32(p[j]);
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[b][j] = 4 * lane + j < nc[b] ? to_f32(xb[j]) : 0.0f;
+                for (int j = 0; j < 4; ++j) v[b][j] = at + j < nc ? to_f32(xb[b * QB + j]) : 0.0f;
             }
         }
 #pragma unroll
@@ -247,41 +241,40 @@ __global__ void __launch_bounds__(256) k_quantize_rows_any(const T *__restrict__
             const float a = fmaxf(fmaxf(kTiny, fmaxf(fabsf(v[b][0]), fabsf(v[b][1]))), fmaxf(fabsf(v[b][2]), fabsf(v[b][3])));
             m[b] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));  // (positive: ordered as its bits)
         }
-        const int mine = lane % NB;
-        const float mm = mine == 0 ? m[0] : mine == 1 ? m[1] : mine == 2 ? m[2] : m[3];
+        const float mm = (lane & 2) ? (lane & 1 ? m[3] : m[2]) : (lane & 1 ? m[1] : m[0]);
         const Factor fm = factor<T>(mm);
-        const float sm = __fdiv_rn(mm, kE4M3Max);
+        if (lane < NB && lane * QB < nc) sb[lane] = __fdiv_rn(mm, kE4M3Max);
         uint32_t w[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const Factor f{__shfl_sync(0xffffffffu, fm.inv, b), __shfl_sync(0xffffffffu, fm.rest, b)};
+            const Factor f{__shfl_sync(0xffffffffu, fm.inv, b), sizeof(T) == 4 ? __shfl_sync(0xffffffffu, fm.rest, b) : 0.0f};
             w[b] = quant4<T>(v[b][0], v[b][1], v[b][2], v[b][3], f);
-            if (lane == b && nc[b]) scale[(int64_t)row[b] * lds + kb[b]] = sm;
         }
+        const int sh = (int)((uintptr_t)qb & 3);
+        const int full = nc & ~(QB - 1);  // what words cover; the rest of the row leaves as bytes
+        uint8_t *at = qb + 4 * lane - sh;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint8_t *qb = q + (int64_t)row[b] * ldq + kb[b] * QB;
-            const int sh = (int)((uintptr_t)qb & 3);
-            // the word that ends before this lane's: the last lane's or the last block's
+            // the word that ends where this lane's begins: the last lane's or the last block's
             uint32_t before = __shfl_up_sync(0xffffffffu, w[b], 1);
             const uint32_t last = __shfl_sync(0xffffffffu, w[b > 0 ? b - 1 : 0], 31);
-            const bool linked = b > 0 && row[b > 0 ? b - 1 : 0] == row[b] && nc[b > 0 ? b - 1 : 0] == QB && nc[b] == QB;
-            const bool goes_on = b + 1 < NB && row[b + 1 < NB ? b + 1 : b] == row[b] && nc[b + 1 < NB ? b + 1 : b] == QB;
             if (lane == 0) before = last;
-            if (nc[b] == QB) {
-                if (lane > 0 || linked || sh == 0) {
-                    *reinterpret_cast<uint32_t *>(qb + 4 * lane - sh) = __funnelshift_l(before, w[b], 8 * sh);
-                } else {
-                    for (int j = 0; j < 4 - sh; ++j) qb[j] = (uint8_t)(w[b] >> 8 * j);
-                }
-                if (lane == 31 && !goes_on)
-                    for (int j = 4 - sh; j < 4; ++j) qb[124 + j] = (uint8_t)(w[b] >> 8 * j);
-            } else {
+            if (b * QB < full) {
+                if (b > 0 || lane > 0 || sh == 0)
+                    *reinterpret_cast<uint32_t *>(at + b * QB) = __funnelshift_l(before, w[b], 8 * sh);
+                else
+                    for (int j = 0; j < 4 - sh; ++j) qb[j] = (uint8_t)(w[0] >> 8 * j);
+                if (lane == 31 && b * QB + QB == full)
+                    for (int j = 4 - sh; j < 4; ++j) qb[b * QB + 124 + j] = (uint8_t)(w[b] >> 8 * j);
+            } else if (b * QB < nc) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (4 * lane + j < nc[b]) qb[4 * lane + j] = (uint8_t)(w[b] >> 8 * j);
+                    if (b * QB + 4 * lane + j < nc) qb[b * QB + 4 * lane + j] = (uint8_t)(w[b] >> 8 * j);
             }
         }
+        row += srow;
+        run += srun;
+        if (run >= runs) run -= runs, ++row;
     }
 }
 
@@ -373,21 +366,23 @@ int quantize(lonnx_ctx *ctx, const void *xv, int64_t rows, int64_t cols, int64_t
     const int64_t nkb = (cols + QB - 1) / QB;
     cudaStream_t st = ctx->stream;
     if (block_rows == 1) {
-        const int64_t total = rows * nkb, per_cta = 256 / 8;  // (both kernels: 32 blocks a CTA)
-        const unsigned grid = (unsigned)std::min<int64_t>((total + per_cta - 1) / per_cta, (int64_t)ctx->num_sms * 32);
-        // 32-bit indices (one 32-bit division per block) where blocks and columns allow it
-        const bool small = total + (int64_t)grid * per_cta * 2 < (1ll << 31) && cols < (1ll << 30);
-        const bool x4 = ((uintptr_t)x & (4 * sizeof(T) - 1)) == 0 && ldx % 4 == 0;
-        if (vec && small)
-            k_quantize_rows<T, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
-        else if (vec)
-            k_quantize_rows<T, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
-        else if (small && x4)
-            k_quantize_rows_any<T, true, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
-        else if (small)
-            k_quantize_rows_any<T, false, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
-        else
-            k_quantize_rows_any<T, false, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        if (vec) {
+            // the CTAs that an SM holds at once (by registers), each walking over blocks
+            const int64_t total = rows * nkb;
+            const unsigned grid = (unsigned)std::min<int64_t>((total + 31) / 32, ctx->num_sms * (sizeof(T) == 4 ? 4 : 3));
+            // 32-bit indices where blocks and columns allow it
+            if (total + grid * 64ll < (1ll << 31) && cols < (1ll << 30))
+                k_quantize_rows<T, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
+            else
+                k_quantize_rows<T, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        } else {
+            const int64_t total = rows * ((nkb + 3) / 4);
+            const unsigned grid = (unsigned)std::min<int64_t>((total + 7) / 8, ctx->num_sms * 4);
+            if (((uintptr_t)x & (4 * sizeof(T) - 1)) == 0 && ldx % 4 == 0)
+                k_quantize_rows_any<T, true><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+            else
+                k_quantize_rows_any<T, false><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
+        }
     } else {
         const int64_t total = (rows + QB - 1) / QB * nkb;
         const unsigned grid = (unsigned)std::min<int64_t>(total, 1ll << 30);
