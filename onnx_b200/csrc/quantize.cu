@@ -282,9 +282,10 @@ __global__ void __launch_bounds__(256, 4) k_quantize_rows_any(const T *__restric
 // values a thread) while the maximum crosses the CTA.
 constexpr int kBlockThreads = 512;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kBlockThreads, 2) k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int64_t rows,
-                                                         int64_t cols, uint8_t *__restrict__ q, int64_t ldq,
-                                                         float *__restrict__ scale, int64_t lds) {
+__global__ void __launch_bounds__(kBlockThreads, VEC && sizeof(T) == 2 ? 3 : 2)
+    k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int64_t rows, int64_t cols, uint8_t *__restrict__ q,
+                      int64_t ldq, float *__restrict__ scale, int64_t lds) {
+    // VEC: a lane's elements are 16-byte vectors, kept as they come; otherwise 4 elements, 32 apart
     constexpr int VN = VEC ? 16 / (int)sizeof(T) : 4;
     constexpr int LANES = QB / VN, TALL = kBlockThreads / LANES;  // rows per step
     constexpr int STEPS = QB / TALL;
@@ -296,36 +297,30 @@ __global__ void __launch_bounds__(kBlockThreads, 2) k_quantize_blocks(const T *_
         const T *xb = x + rb * QB * ldx + kb * QB;
         uint8_t *qb = q + rb * QB * ldq + kb * QB;
         const int nr = (int)min((int64_t)QB, rows - rb * QB), nc = (int)min((int64_t)QB, cols - kb * QB);
-        float v[STEPS][VN];
-        float m = kTiny;
+        T part[STEPS][VN];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int r = r0 + s * TALL;
             const T *xr = xb + (int64_t)r * ldx;
-            if constexpr (VEC) {
-                const int at = lane * VN;
-                if (r < nr && at + VN <= nc) {
-                    unpack<T>(__ldcs(reinterpret_cast<const uint4 *>(xr + at)), v[s]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VN; ++j) v[s][j] = r < nr && at + j < nc ? to_f32(xr[at + j]) : 0.0f;
-                }
+            if (VEC && r < nr && lane * VN + VN <= nc) {
+                *reinterpret_cast<uint4 *>(part[s]) = __ldcs(reinterpret_cast<const uint4 *>(xr + lane * VN));
             } else {
 #pragma unroll
-                for (int j = 0; j < VN; ++j)
-                    v[s][j] = r < nr && lane + 32 * j < nc ? to_f32(xr[lane + 32 * j]) : 0.0f;
+                for (int j = 0; j < VN; ++j) {
+                    const int at = VEC ? lane * VN + j : lane + 32 * j;
+                    part[s][j] = r < nr && at < nc ? xr[at] : T(0.0f);
+                }
             }
         }
+        float m = kTiny;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(v[s][j]));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int j = 0; j < VN; ++j) m = fmaxf(m, fabsf(to_f32(part[s][j])));
+        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // (positive: ordered as its bits)
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kBlockThreads / 32; ++w) m = fmaxf(m, red[w]);
+        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(red[threadIdx.x % (kBlockThreads / 32)])));
         __syncthreads();
         const Factor f = factor<T>(m);
         if (threadIdx.x == 0) scale[rb * lds + kb] = __fdiv_rn(m, kE4M3Max);
@@ -337,21 +332,17 @@ __global__ void __launch_bounds__(kBlockThreads, 2) k_quantize_blocks(const T *_
             uint32_t w[VN / 4];
 #pragma unroll
             for (int j = 0; j < VN / 4; ++j)
-                w[j] = quant4<T>(v[s][4 * j], v[s][4 * j + 1], v[s][4 * j + 2], v[s][4 * j + 3], f);
-            if constexpr (VEC) {
-                const int at = lane * VN;
-                if (at + VN <= nc) {
-                    if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qr + at) = w[0];
-                    else *reinterpret_cast<uint2 *>(qr + at) = make_uint2(w[0], w[VN / 4 - 1]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VN; ++j)
-                        if (at + j < nc) qr[at + j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
-                }
+                w[j] = quant4<T>(to_f32(part[s][4 * j]), to_f32(part[s][4 * j + 1]), to_f32(part[s][4 * j + 2]),
+                                 to_f32(part[s][4 * j + 3]), f);
+            if (VEC && lane * VN + VN <= nc) {
+                if constexpr (VN == 4) *reinterpret_cast<uint32_t *>(qr + lane * VN) = w[0];
+                else *reinterpret_cast<uint2 *>(qr + lane * VN) = make_uint2(w[0], w[VN / 4 - 1]);
             } else {
 #pragma unroll
-                for (int j = 0; j < VN; ++j)
-                    if (lane + 32 * j < nc) qr[lane + 32 * j] = (uint8_t)(w[0] >> 8 * j);
+                for (int j = 0; j < VN; ++j) {
+                    const int at = VEC ? lane * VN + j : lane + 32 * j;
+                    if (at < nc) qr[at] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+                }
             }
         }
     }
