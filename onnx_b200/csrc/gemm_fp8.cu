@@ -122,9 +122,9 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 //                time through 4 KB of shared memory per warp and out by TMA (or, where rows of C do not start on 16 bytes, by element
 //                stores that coalesce along rows)
 //   warp 16      TMA producer
-//   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM): waits and
-//                loop around a block's four MMAs took a single issuer 350 of
-//                860 cycles
+//   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM); with 256
+//                columns a block's MMAs take the tensor cores as long as the
+//                waits and the loop around them, and warp 17 issues all
 //   warp 19      the block's scales: sA[m, b] * sB[n / 128, b] of the tile's 128
 //                rows and BN / 128 column blocks into shared memory, one slot
 //                per TMEM buffer, under the same barriers
@@ -133,12 +133,15 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 // one set runs beside the other's blocks.
 // The drain warps take registers from the other four (setmaxnreg): 512 x 112 +
 // 128 x 32 = 640 x 96, the launch's.
-template <int BN>
+template <int BN, int ES>
 struct Wide {
     static constexpr int STAGE = kTile + BN * KB;
-    static constexpr int S = BN == 256 ? 3 : 5;
     static constexpr int SETS = 256 / BN, BUFS = 2 * SETS;
-    static constexpr int STAGING = 16 * 4096;
+    static constexpr int PIECES = 1;  // of 128 bytes x 32 rows, per warp in the epilogue
+    static constexpr int S = BN == 256 ? 3 : 4;
+    // With two issuers a ring slot has to belong to one of them (see the MMA warps).
+    static constexpr int ISSUERS = S % 2 == 0 ? 2 : 1;
+    static constexpr int STAGING = 16 * 4096 * PIECES;
     static constexpr int SCALES = BUFS * BN * 4;  // a slot per buffer: BN / 128 column blocks x 128 rows
     static constexpr int BARS = 2 * S + 2 * BUFS + 1;
     static constexpr int SMEM = S * STAGE + STAGING + SCALES + BARS * 8 + 8;
@@ -166,7 +169,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const __grid_constant__ CUtensorMap mapC, const float *__restrict__ sA, int64_t ldsA,
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int *flags) {
-    using W = Wide<BN>;
+    using W = Wide<BN, (int)sizeof(T)>;
     constexpr int GROUP = BY_TMA ? 16 : 1;
     constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             mbar_init(tfull(b), 1 + 32);  // the MMAs' commit and the scale warp's lanes
             mbar_init(tempty(b), 16 / SETS);
         }
-        mbar_init(drained, 2);
+        mbar_init(drained, 2);  // a commit of each MMA warp
         fence_mbar_init();
     }
     if (warp == W_MMA) {
@@ -232,17 +235,22 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             const uint64_t desc0 = smem_desc_sw128(smem_u32(base));
             // Issuer e takes blocks e, e + 2, .. of the ring's order.  A parity wait
-            // must not be two phases ahead of its barrier: the ring's order holds
-            // the issuers within S blocks of each other, and full() is waited for
-            // before tempty(), which then is at most one phase ahead: the block two
-            // before in its buffer is this issuer's own, or at least S before.
+            // must not be two phases ahead of its barrier, or it returns at once.
+            // full(): loads land in any order, so block i - S need not have landed
+            // when a later one has; but S is even, so the issuer that waits for
+            // block i in slot i % S is the one that waited for block i - S there.
+            // tempty(): it is waited for after full(), and block i's load was
+            // issued after the MMAs of blocks up to i - S ended.  The block two
+            // before in the same TMEM buffer is this issuer's own or (sets of an
+            // odd number of blocks, at least 3) 5 or more before in the ring, so it
+            // has passed its own wait, and this one is at most one phase ahead.
             int js[2] = {0, 0}, i = 0;  // blocks of each set, blocks of all
             for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
                 const int set = SETS == 2 ? n & 1 : 0;
                 int j = js[set];
                 js[set] += nkb;
                 for (int b = 0; b < nkb; ++b, ++j, ++i) {
-                    if ((i & 1) != warp - W_MMA) continue;
+                    if (i % W::ISSUERS != warp - W_MMA) continue;
                     const int s = i % S, buf = 2 * set + (j & 1);
                     const bool ready = mbar_wait(full(s), (i / S) & 1, abort_flag) &&
                                        mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag);
@@ -366,25 +374,28 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[i + u]);
                 return *reinterpret_cast<const uint4 *>(out);
             };
-            uint8_t *stage = staging + warp * 4096;
+            uint8_t *stage = staging + warp * (W::STAGING / 16);
             if constexpr (BY_TMA) {
                 // 128 bytes of each of the warp's 32 rows at a time: one piece is
                 // computed in registers while the last one leaves shared memory
                 constexpr int PIECE = 128 / (int)sizeof(T);
 #pragma unroll
-                for (int p = 0; p < COLS / PIECE; ++p) {
+                for (int p0 = 0; p0 < COLS / PIECE; p0 += W::PIECES) {
 #pragma unroll
-                    for (int i = p * PIECE; i < (p + 1) * PIECE; i += 32) finish(i);
+                    for (int i = p0 * PIECE; i < (p0 + W::PIECES) * PIECE; i += 32) finish(i);
                     if (lane == 0) bulk_wait_group_read0();
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)  // 16-byte chunks of this lane's row, 128B-swizzled
-                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack(p * PIECE + c * CN);
+                    for (int c = 0; c < 8 * W::PIECES; ++c)  // 16-byte chunks of this lane's row, 128B-swizzled
+                        *reinterpret_cast<uint4 *>(stage + c / 8 * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+                            pack(p0 * PIECE + c * CN);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    const int col = col0 + p * PIECE;
-                    if (lane == 0 && col < N && row0 < M) {
-                        tma_store_2d(&mapC, smem_u32(stage), col, row0);
+                    if (lane == 0 && row0 < M) {
+#pragma unroll
+                        for (int p = 0; p < W::PIECES; ++p)
+                            if (col0 + (p0 + p) * PIECE < N)
+                                tma_store_2d(&mapC, smem_u32(stage + p * 4096), col0 + (p0 + p) * PIECE, row0);
                         bulk_commit_group();
                     }
                 }
@@ -734,7 +745,7 @@ struct Problem {
 
 template <int BN, typename T, bool BY_TMA>
 int launch_wide(lonnx_ctx *ctx, const Problem &p) {
-    using W = Wide<BN>;
+    using W = Wide<BN, (int)sizeof(T)>;
     CUtensorMap ma, mb, mc;
     int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, BM);
     if (!rc) rc = tile_map(&mb, p.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.ldb, BN);

@@ -190,7 +190,7 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (1, 1000, 257), (2, 129, 4096), (7, 384, 384
           (17, 513, 640), (31, 65, 33), (32, 2000, 384), (33, 640, 1152), (64, 300, 2048), (65, 1536, 384),
           (127, 127, 127), (128, 256, 128), (129, 257, 129), (200, 1000, 1001), (256, 256, 8192), (300, 4100, 384),
           (777, 1000, 1111), (1024, 192, 96), (1500, 2100, 300), (2048, 2300, 2100), (1700, 1900, 1100),
-          (2600, 4000, 130), (4000, 5000, 520)]
+          (2600, 4000, 130), (4000, 5000, 520), (19000, 380, 640), (20000, 640, 300)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
