@@ -122,9 +122,9 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 //                time through 4 KB of shared memory per warp and out by TMA (or, where rows of C do not start on 16 bytes, by element
 //                stores that coalesce along rows)
 //   warp 16      TMA producer
-//   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM); with 256
-//                columns a block's MMAs take the tensor cores as long as the
-//                waits and the loop around them, and warp 17 issues all
+//   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM): one's waits
+//                run while the other issues (a single issuer: 2048^3 in 14.5 us
+//                instead of 13.0)
 //   warp 19      the block's scales: sA[m, b] * sB[n / 128, b] of the tile's 128
 //                rows and BN / 128 column blocks into shared memory, one slot
 //                per TMEM buffer, under the same barriers
@@ -133,17 +133,15 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 // one set runs beside the other's blocks.
 // The drain warps take registers from the other four (setmaxnreg): 512 x 112 +
 // 128 x 32 = 640 x 96, the launch's.
-template <int BN, int ES>
+template <int BN>
 struct Wide {
     static constexpr int STAGE = kTile + BN * KB;
     static constexpr int SETS = 256 / BN, BUFS = 2 * SETS;
-    static constexpr int PIECES = 1;  // of 128 bytes x 32 rows, per warp in the epilogue
     static constexpr int S = BN == 256 ? 3 : 4;
-    // With two issuers a ring slot has to belong to one of them (see the MMA warps).
-    static constexpr int ISSUERS = S % 2 == 0 ? 2 : 1;
-    static constexpr int STAGING = 16 * 4096 * PIECES;
+    static constexpr bool TURNS = S % 2 != 0;  // of the two issuers (see there)
+    static constexpr int STAGING = 16 * 4096;  // 128 bytes x 32 rows per warp in the epilogue
     static constexpr int SCALES = BUFS * BN * 4;  // a slot per buffer: BN / 128 column blocks x 128 rows
-    static constexpr int BARS = 2 * S + 2 * BUFS + 1;
+    static constexpr int BARS = 2 * S + 2 * BUFS + 3;
     static constexpr int SMEM = S * STAGE + STAGING + SCALES + BARS * 8 + 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const __grid_constant__ CUtensorMap mapC, const float *__restrict__ sA, int64_t ldsA,
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int *flags) {
-    using W = Wide<BN, (int)sizeof(T)>;
+    using W = Wide<BN>;
     constexpr int GROUP = BY_TMA ? 16 : 1;
     constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
@@ -181,7 +179,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     auto empty = [&](int s) { return bars + 8 * (S + s); };
     auto tfull = [&](int b) { return bars + 8 * (2 * S + b); };
     auto tempty = [&](int b) { return bars + 8 * (2 * S + W::BUFS + b); };
-    const uint32_t drained = bars + 8 * (2 * S + 2 * W::BUFS);
+    auto turn = [&](int e) { return bars + 8 * (2 * S + 2 * W::BUFS + e); };
+    const uint32_t drained = bars + 8 * (2 * S + 2 * W::BUFS + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bar0 + W::BARS);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar0 + W::BARS) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,6 +195,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             mbar_init(tfull(b), 1 + 32);  // the MMAs' commit and the scale warp's lanes
             mbar_init(tempty(b), 16 / SETS);
         }
+        mbar_init(turn(0), 1);
+        mbar_init(turn(1), 1);
         mbar_init(drained, 2);  // a commit of each MMA warp
         fence_mbar_init();
     }
@@ -236,24 +237,29 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             const uint64_t desc0 = smem_desc_sw128(smem_u32(base));
             // Issuer e takes blocks e, e + 2, .. of the ring's order.  A parity wait
             // must not be two phases ahead of its barrier, or it returns at once.
-            // full(): loads land in any order, so block i - S need not have landed
-            // when a later one has; but S is even, so the issuer that waits for
-            // block i in slot i % S is the one that waited for block i - S there.
-            // tempty(): it is waited for after full(), and block i's load was
-            // issued after the MMAs of blocks up to i - S ended.  The block two
-            // before in the same TMEM buffer is this issuer's own or (sets of an
-            // odd number of blocks, at least 3) 5 or more before in the ring, so it
-            // has passed its own wait, and this one is at most one phase ahead.
+            // full(): loads land in any order, so a block may be there before the one
+            // S earlier, in the same slot.  With S even that one was this issuer's,
+            // which has waited for it; with S odd the issuers take turns at this wait
+            // (turn), and it is always for the block after the last one seen.
+            // tempty(): the block two before in its TMEM buffer is this issuer's own
+            // or, where sets have an odd number of blocks, 5 or more before in the
+            // ring, and this block's load waited for the MMAs up to S before it.
+            const int e = warp - W_MMA;
             int js[2] = {0, 0}, i = 0;  // blocks of each set, blocks of all
             for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
                 const int set = SETS == 2 ? n & 1 : 0;
                 int j = js[set];
                 js[set] += nkb;
                 for (int b = 0; b < nkb; ++b, ++j, ++i) {
-                    if (i % W::ISSUERS != warp - W_MMA) continue;
+                    if ((i & 1) != e) continue;
                     const int s = i % S, buf = 2 * set + (j & 1);
-                    const bool ready = mbar_wait(full(s), (i / S) & 1, abort_flag) &&
-                                       mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag);
+                    bool ready = (!W::TURNS || mbar_wait(turn(e), ((i >> 1) & 1) ^ (e ^ 1), abort_flag)) &&
+                                 mbar_wait(full(s), (i / S) & 1, abort_flag);
+                    if (W::TURNS) {
+                        if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+                        if (lane == 0) mbar_arrive(turn(e ^ 1));
+                    }
+                    ready = ready && mbar_wait(tempty(buf), ((j >> 1) & 1) ^ 1, abort_flag);
                     if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
                     tc_fence_after();
                     const uint64_t da = desc0 + (uint32_t)(s * (W::STAGE / 16)), db = da + kTile / 16;
@@ -374,28 +380,25 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 for (int u = 0; u < CN; ++u) out[u] = from_f32<T>(acc[i + u]);
                 return *reinterpret_cast<const uint4 *>(out);
             };
-            uint8_t *stage = staging + warp * (W::STAGING / 16);
+            uint8_t *stage = staging + warp * 4096;
             if constexpr (BY_TMA) {
                 // 128 bytes of each of the warp's 32 rows at a time: one piece is
                 // computed in registers while the last one leaves shared memory
                 constexpr int PIECE = 128 / (int)sizeof(T);
 #pragma unroll
-                for (int p0 = 0; p0 < COLS / PIECE; p0 += W::PIECES) {
+                for (int p = 0; p < COLS / PIECE; ++p) {
 #pragma unroll
-                    for (int i = p0 * PIECE; i < (p0 + W::PIECES) * PIECE; i += 32) finish(i);
+                    for (int i = p * PIECE; i < (p + 1) * PIECE; i += 32) finish(i);
                     if (lane == 0) bulk_wait_group_read0();
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 8 * W::PIECES; ++c)  // 16-byte chunks of this lane's row, 128B-swizzled
-                        *reinterpret_cast<uint4 *>(stage + c / 8 * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
-                            pack(p0 * PIECE + c * CN);
+                    for (int c = 0; c < 8; ++c)  // 16-byte chunks of this lane's row, 128B-swizzled
+                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack(p * PIECE + c * CN);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && row0 < M) {
-#pragma unroll
-                        for (int p = 0; p < W::PIECES; ++p)
-                            if (col0 + (p0 + p) * PIECE < N)
-                                tma_store_2d(&mapC, smem_u32(stage + p * 4096), col0 + (p0 + p) * PIECE, row0);
+                    const int col = col0 + p * PIECE;
+                    if (lane == 0 && col < N && row0 < M) {
+                        tma_store_2d(&mapC, smem_u32(stage), col, row0);
                         bulk_commit_group();
                     }
                 }
@@ -745,7 +748,7 @@ struct Problem {
 
 template <int BN, typename T, bool BY_TMA>
 int launch_wide(lonnx_ctx *ctx, const Problem &p) {
-    using W = Wide<BN, (int)sizeof(T)>;
+    using W = Wide<BN>;
     CUtensorMap ma, mb, mc;
     int rc = tile_map(&ma, p.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.M, p.K, p.lda, BM);
     if (!rc) rc = tile_map(&mb, p.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.N, p.K, p.ldb, BN);
@@ -827,7 +830,7 @@ int launch_split(lonnx_ctx *ctx, const Problem &p, int parts) {
 struct Choice {
     int width, parts;  // 256, 128: wide tiles; 64, 32, 16: rows of A of a split tile
 };
-Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
+Choice choose(int64_t M, int64_t N, int64_t K, int es, int sms) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     const double l2 = 7.5e6;  // bytes a microsecond
     const int64_t nkb = up(K, KB);
@@ -841,7 +844,8 @@ Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
     };
     for (int bn : {256, 128}) {
         const int64_t tiles = up(M, BM) * up(N, bn), rounds = up(tiles, sms);
-        const double block = bn == 256 ? 0.58 : tiles > sms ? 0.39 : 0.31, epilogue = bn == 256 ? 2.3 : 1.2;
+        const double block = bn == 256 ? 0.58 : tiles > sms ? 0.36 : 0.31;
+        const double epilogue = bn == 256 ? (es == 4 ? 2.6 : 1.5) : (es == 4 ? 1.1 : 0.8);
         offer(bn, 1, std::max(rounds * (nkb * block + epilogue), tiles * nkb * double(kTile + bn * KB) / l2));
     }
     // CTAs that run at once in clusters of 1, 2, 4, 8 (a GPC has 16 to 18 SMs)
@@ -870,7 +874,7 @@ int launch(lonnx_ctx *ctx, const Problem &p) {
         LONNX_CHECK_LAUNCH(ctx);
         return LONNX_OK;
     }
-    const Choice c = choose(p.M, p.N, p.K, ctx->num_sms);
+    const Choice c = choose(p.M, p.N, p.K, (int)sizeof(T), ctx->num_sms);
     switch (c.width) {
         case 256: return launch_wide<256, T>(ctx, p);
         case 128: return launch_wide<128, T>(ctx, p);

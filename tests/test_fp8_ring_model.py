@@ -1,8 +1,8 @@
 """A model of the wide 8-bit product kernel's barriers (csrc/gemm_fp8.cu): its
 warps as generators, stepped in random order, with parity waits answered as an
 mbarrier answers them and loads that land in any order.  It holds the kernel's
-ring sizes and issuer counts sound, and shows that two issuers over an odd
-number of slots are not."""
+rings sound, and shows that over an odd number of slots two issuers have to take
+turns at the wait for a load."""
 import os
 import random
 import re
@@ -26,10 +26,11 @@ class Bar:
         return (self.phase & 1) != parity
 
 
-def simulate(sets, slots, issuers, blocks, tiles, seed):
+def simulate(sets, slots, blocks, tiles, seed, turns=True):
     rnd = random.Random(seed)
     full, empty = [Bar(1) for _ in range(slots)], [Bar(1) for _ in range(slots)]
     tfull, tempty = [Bar(2) for _ in range(2 * sets)], [Bar(1) for _ in range(2 * sets)]
+    turn = [Bar(1), Bar(1)]
     ring, acc, scales = [None] * slots, [None] * (2 * sets), [None] * (2 * sets)
     queue, flying, drained, loaded = [], [], [], []
 
@@ -60,9 +61,12 @@ def simulate(sets, slots, issuers, blocks, tiles, seed):
 
     def issue(e):
         for i, s, j, what in order():
-            if i % issuers == e:
+            if i & 1 == e:
+                while turns and not turn[e].passed((i >> 1 & 1) ^ e ^ 1):
+                    yield
                 while not full[i % slots].passed(i // slots & 1):
                     yield
+                turn[e ^ 1].arrive()
                 yield
                 buf = 2 * s + (j & 1)
                 while not tempty[buf].passed((j >> 1 & 1) ^ 1):
@@ -103,7 +107,7 @@ def simulate(sets, slots, issuers, blocks, tiles, seed):
                 for _ in range(rnd.randrange(30) if what[1] == blocks - 1 else 0):  # the epilogue
                     yield
 
-    actors = [load(), land(), tensor(), scale()] + [issue(e) for e in range(issuers)] + [drain(s) for s in range(sets)]
+    actors = [load(), land(), tensor(), scale()] + [issue(e) for e in range(2)] + [drain(s) for s in range(sets)]
     weights, steps = None, 0
     while actors:
         if weights is None or rnd.random() < 0.01:
@@ -119,28 +123,28 @@ def simulate(sets, slots, issuers, blocks, tiles, seed):
 
 
 def kernel_configurations():
-    """(sets, slots, issuers) of the 256- and 128-column tiles, from the source."""
+    """(sets, slots) of the 256- and 128-column tiles, from the source."""
     src = open(os.path.join(ROOT, "onnx_b200", "csrc", "gemm_fp8.cu")).read()
+    assert "TURNS = S % 2 != 0;" in src
     m = re.search(r"static constexpr int S = BN == 256 \? (\d+) : (\d+);", src)
-    assert m and "ISSUERS = S % 2 == 0 ? 2 : 1" in src
-    return [(256 // bn, int(s), 2 if int(s) % 2 == 0 else 1) for bn, s in ((256, m.group(1)), (128, m.group(2)))]
+    return [(256 // bn, int(s)) for bn, s in ((256, m.group(1)), (128, m.group(2)))]
 
 
-@pytest.mark.parametrize("sets, slots, issuers", kernel_configurations())
+@pytest.mark.parametrize("sets, slots", kernel_configurations())
 @pytest.mark.parametrize("blocks", [1, 2, 3, 4, 5, 7])
-def test_rings_are_sound(sets, slots, issuers, blocks):
+def test_rings_are_sound(sets, slots, blocks):
     for tiles in (1, 2, 7):
         for seed in range(12):
-            simulate(sets, slots, issuers, blocks, tiles, seed)
+            simulate(sets, slots, blocks, tiles, seed, turns=slots % 2 != 0)
 
 
-def test_two_issuers_need_an_even_ring():
-    def fails(slots):
+def test_issuers_of_an_odd_ring_take_turns():
+    def fails(slots, turns):
         n = 0
         for seed in range(60):
             try:
-                simulate(2, slots, 2, 3, 13, seed)
+                simulate(2, slots, 3, 13, seed, turns)
             except AssertionError:
                 n += 1
         return n
-    assert fails(3) and not fails(4)
+    assert fails(3, False) and not fails(3, True) and not fails(4, False)
