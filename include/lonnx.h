@@ -176,8 +176,11 @@ LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64
  * or NULL.  C: [M, N] of type dtypeC (float, float16, bfloat16) at ldc
  * elements; what lies past a row's end is left as it is.  Each block's product
  * is summed by the tensor cores, blocks are scaled and summed in fp32, and the
- * result is rounded to C's type once, after the epilogue.  Runs without
- * workspace.  lonnx_gemm_f32's counterpart for quantised weights. */
+ * result is rounded to C's type once, after the epilogue (lonnx_gemm_f32's,
+ * whose ReLU gives 0 for NaN).  K = 0 gives the bias through the activation.
+ * Sizes up to 2^30.  The order of the sums is fixed by the sizes: the same
+ * call gives the same bits.  Runs without workspace.  lonnx_gemm_f32's
+ * counterpart for quantised weights. */
 LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t lda, const float *scaleA, int64_t ldsA,
                              const void *B, int64_t ldb, const float *scaleB, int64_t ldsB, const float *bias,
                              void *C, int dtypeC, int64_t ldc, int M, int N, int K, int epilogue);

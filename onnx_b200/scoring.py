@@ -158,7 +158,7 @@ def token_logprobs(logits: DeviceTensor, targets: DeviceTensor | None = None, k:
     if k and (ptr["top_logprob"] is None or ptr["top_id"] is None):
         raise ValueError("out: top_logprob and top_id are both needed with k > 0")
     rc = _logprobs(ctx.handle, logits.ptr, ONNX_DTYPE[logits.dtype], rows, vocab, ld,
-                   None if targets is None else targets.ptr, temperature, ptr["logprob"], ptr["entropy"], k,
+                   None if targets is None else targets.ptr, float(temperature), ptr["logprob"], ptr["entropy"], k,
                    ptr["top_logprob"], ptr["top_id"])
     if rc:
         N.check(rc)

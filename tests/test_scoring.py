@@ -110,6 +110,7 @@ def logprobs(x=4096, dtype=1, rows=4, vocab=100, ld=100, targets=4096, temperatu
     (quantize, dict(), BADARG, "null context"),
     (gemm, dict(dtype=17), UNSUPPORTED, "output type"),
     (gemm, dict(K=-1), BADARG, "negative"),
+    (gemm, dict(M=(1 << 30) + 1), UNSUPPORTED, "2^30"),
     (gemm, dict(epi=3), BADARG, "epilogue"),
     (gemm, dict(lda=192), SHAPE, "leading dimension"),
     (gemm, dict(ldc=7), SHAPE, "leading dimension"),
