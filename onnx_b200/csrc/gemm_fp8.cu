@@ -125,7 +125,8 @@ __device__ __forceinline__ void load_scales(float (&s)[4], const float *row, int
 //   warps 0-15   drain: each thread one row x 64 columns in registers (four
 //                warps a scheduler: the TMEM loads of one hide behind the FMAs
 //                of the others); then the epilogue, 128 bytes of a row at a
-//                time through 4 KB of shared memory per warp and out by TMA (or, where rows of C do not start on 16 bytes, by element
+//                time through 4 KB of shared memory per warp and out by TMA (or,
+//                where rows of C do not start and end on 16 bytes, by element
 //                stores that coalesce along rows)
 //   warp 16      TMA producer
 //   warps 17, 18 MMA issuers of every other block (warp 17 has TMEM): one's waits
@@ -156,9 +157,9 @@ constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 19;
 
 // Tiles in groups of `GROUP` rows of tiles, column by column within a group, so
 // that the CTAs at work share both operands' tiles in L2.  Where C leaves by
-// element stores, its rows do not start on sectors, and a group is one row of
-// tiles: two neighbours' halves of a sector meet in L2 (18651 x 17257 floats
-// written as tiles: 407 us in groups of 16, 351 row by row).
+// element stores, its rows do not start on sectors, and a group is 4 rows: two
+// neighbours' halves of a sector meet in L2 (18651 x 17257 x 78 to bfloat16: 235
+// us, 299 in groups of 16; 1000 x 30001 x 2000 to halves: 105, 113 row by row).
 template <int GROUP>
 __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int &tm, int &tn) {
     const int per = GROUP * tiles_n, g = t / per, first = g * GROUP;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int *flags) {
     using W = Wide<BN>;
-    constexpr int GROUP = BY_TMA ? 16 : 1;
+    constexpr int GROUP = BY_TMA ? 16 : 4;
     constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *staging = base + S * W::STAGE;
@@ -787,7 +788,9 @@ int launch_wide(lonnx_ctx *ctx, const Problem &p) {
 
 template <int BN, typename T>
 int launch_wide(lonnx_ctx *ctx, const Problem &p) {
-    const bool by_tma = ((uintptr_t)p.C & 15) == 0 && p.ldc * (int64_t)sizeof(T) % 16 == 0;
+    // (a TMA store ends on 16 bytes: where N does not, it would write past the row's end)
+    const bool by_tma = ((uintptr_t)p.C & 15) == 0 && p.ldc * (int64_t)sizeof(T) % 16 == 0 &&
+                        p.N * (int64_t)sizeof(T) % 16 == 0;
     return by_tma ? launch_wide<BN, T, true>(ctx, p) : launch_wide<BN, T, false>(ctx, p);
 }
 

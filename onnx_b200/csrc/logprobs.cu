@@ -564,8 +564,14 @@ __global__ void __launch_bounds__(32 * NW, (TOP ? 32 : 24) / NW) k_logprobs_cta(
 template <int NW, typename T, bool TOP>
 int launch_cta(lonnx_ctx *ctx, const T *x, const Args &g, int parts) {
     auto kernel = k_logprobs_cta<NW, T, TOP>;
+    const unsigned grid = (unsigned)(std::min<int64_t>(g.rows, (1 << 30) / parts) * parts);
+    if (parts == 1) {
+        kernel<<<grid, 32 * NW, 0, ctx->stream>>>(x, g);
+        LONNX_CHECK_LAUNCH(ctx);
+        return LONNX_OK;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(g.rows, (1 << 30) / parts) * parts));
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(32 * NW);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];

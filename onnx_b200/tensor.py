@@ -23,6 +23,8 @@ ONNX_DTYPE = {np.dtype(np.float16): 10, BFLOAT16: 16, FLOAT8E4M3: 17,
               np.dtype(np.float32): 1, np.dtype(np.int64): 7, np.dtype(np.int32): 6,
               np.dtype(np.uint8): 2, np.dtype(np.bool_): 9, np.dtype(np.float64): 11}
 NP_DTYPE = {v: k for k, v in ONNX_DTYPE.items()}
+# what np.dtype() answers for the usual types, without its cost
+_DTYPES = {**{d: d for d in ONNX_DTYPE}, **{d.type: d for d in ONNX_DTYPE if d.type is not np.void}}
 
 
 class Context:
@@ -90,7 +92,7 @@ class DeviceTensor:
     def __init__(self, ctx: Context, shape, dtype, ptr=None, owner=None):
         self.ctx = ctx
         self.shape = tuple(map(int, shape))
-        self.dtype = np.dtype(dtype)
+        self.dtype = _DTYPES.get(dtype) or np.dtype(dtype)
         if ptr is None:
             owner = _Allocation(ctx, self.nbytes)
             ptr = owner.ptr

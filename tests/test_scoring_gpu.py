@@ -226,7 +226,8 @@ def test_product_bias_and_activation(tctx, m, n, k, act, dtype):
 
 
 @pytest.mark.parametrize("m, n, k, lda, ldb, ldc", [(3, 129, 200, 256, 208, 131), (150, 300, 200, 208, 512, 304),
-                                                     (260, 515, 390, 400, 416, 517), (40, 515, 390, 400, 416, 600)])
+                                                     (260, 515, 390, 400, 416, 517), (40, 515, 390, 400, 416, 600),
+                                                     (500, 495, 390, 400, 400, 496), (700, 1463, 24, 32, 32, 1464)])
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_product_strides(tctx, m, n, k, lda, ldb, ldc, dtype):
     a, sa, b, sb = fp8_operands(m, n, k, seed=4, lda=lda, ldb=ldb)
