@@ -494,18 +494,24 @@ def test_scoring_captured_and_replayed():
         assert all(np.array_equal(replayed[n], fresh[n].to_host()) for n in replayed)
 
 
-def test_scoring_on_two_streams(tctx):
-    """Two contexts on one GPU, working at the same time on their own streams."""
+@pytest.mark.parametrize("tokens, other", [(40, 40), (1, 1500), (1500, 200)])
+def test_scoring_on_two_streams(tctx, tokens, other):
+    """Two contexts on one GPU, working at the same time on their own streams,
+    also with kernels that share an SM's tensor memory."""
     a, b = Context(0), Context(0)
-    h, w = randn(40, 640, seed=1), randn(3001, 640, seed=2) * 0.05
-    target = torch.randint(0, 3001, (40,), generator=gen(3), device="cuda")
+    h, w = randn(max(tokens, other), 640, seed=1), randn(3001, 640, seed=2) * 0.05
+    target = torch.randint(0, 3001, (max(tokens, other),), generator=gen(3), device="cuda")
     torch.cuda.synchronize()
     heads = [scoring.quantize_fp8(dev(c, w), block_rows=128) for c in (a, b)]
-    runs = [[score(c, h, head, target, 4)[0] for c, head in zip((a, b), heads)] for _ in range(8)]
-    first = {n: t.to_host() for n, t in runs[0][0].items()}
+    sizes = (tokens, other)
+    alone = []
+    for c, head, m in zip((a, b), heads, sizes):
+        alone.append({n: t.to_host() for n, t in score(c, h[:m], head, target[:m], 4)[0].items()})
+        c.sync()
+    runs = [[score(c, h[:m], head, target[:m], 4)[0] for c, head, m in zip((a, b), heads, sizes)] for _ in range(20)]
     for pair in runs:
-        for got in pair:
-            assert all(np.array_equal(first[n], t.to_host()) for n, t in got.items())
+        for got, want in zip(pair, alone):
+            assert all(np.array_equal(want[n], t.to_host()) for n, t in got.items())
 
 
 def test_context_on_a_stream():
