@@ -58,7 +58,11 @@ typedef struct lonnx_ctx lonnx_ctx;
 LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out);
 /* The same on a stream that the caller owns (a cudaStream_t of `device`; NULL
  * is the default stream) and keeps until the context is destroyed: work of
- * the context is then ordered with the caller's own on that stream. */
+ * the context is then ordered with the caller's own on that stream.  Calls
+ * recorded into a CUDA graph of the caller's need their buffers for as long as
+ * the graph is replayed: blocks freed during the recording are kept for it,
+ * later ones are the caller's to keep (and one call outside the recording first
+ * lets the allocator fetch its memory). */
 LONNX_API int lonnx_ctx_create_on_stream(int device, void *stream, lonnx_ctx **out);
 LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx);
 LONNX_API int lonnx_ctx_device(const lonnx_ctx *ctx);

@@ -23,6 +23,11 @@ struct Allocator {
     // cudaMalloc/cudaFree on the execute path.
     std::multimap<size_t, void *> free_blocks;
     std::unordered_map<void *, size_t> live;
+    // Blocks freed while a caller records the stream into a CUDA graph: the graph
+    // has their addresses, so only the same capture may use them again.  They
+    // stay live until the context goes.
+    std::multimap<size_t, void *> captured_blocks;
+    unsigned long long capture_id = 0;
     size_t bytes_reserved = 0;
     size_t limit = 0;  // 0 = none; LONNX_MEM_LIMIT (bytes) caps reservations
 };

@@ -52,9 +52,31 @@ static size_t round_size(size_t b) {
     return (b + g - 1) / g * g;
 }
 
+// The id of the capture that records the context's stream into a caller's CUDA
+// graph; 0 when there is none.
+static unsigned long long caller_capture(lonnx_ctx *ctx) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(ctx->stream, &status, &id) != cudaSuccess) cudaGetLastError();
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 int ctx_alloc(lonnx_ctx *ctx, size_t bytes, void **out) {
     Allocator &A = ctx->alloc;
     const size_t sz = round_size(bytes);
+    if (!A.captured_blocks.empty()) {
+        const unsigned long long id = caller_capture(ctx);
+        if (id && id == A.capture_id) {
+            auto of = A.captured_blocks.find(sz);
+            if (of != A.captured_blocks.end()) {
+                *out = of->second;
+                A.captured_blocks.erase(of);
+                return LONNX_OK;
+            }
+        } else {
+            A.captured_blocks.clear();  // that capture is over: its blocks stay its graph's
+        }
+    }
     auto it = A.free_blocks.find(sz);
     if (it != A.free_blocks.end()) {
         *out = it->second;
@@ -95,6 +117,12 @@ int ctx_free(lonnx_ctx *ctx, void *p) {
     if (it == A.live.end()) return set_error(LONNX_E_BADARG, "lonnx_free: pointer %p not allocated by this context", p);
     if (ctx->capturing) {
         ctx->capture_hold.push_back(p);  // stays live until the captured graph is released
+        return LONNX_OK;
+    }
+    if (const unsigned long long id = caller_capture(ctx)) {
+        if (id != A.capture_id) A.captured_blocks.clear();  // an earlier capture's, its graph's for good
+        A.captured_blocks.emplace(it->second, p);
+        A.capture_id = id;
         return LONNX_OK;
     }
     A.free_blocks.emplace(it->second, p);

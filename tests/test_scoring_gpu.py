@@ -494,6 +494,32 @@ def test_scoring_captured_and_replayed():
         assert all(np.array_equal(replayed[n], fresh[n].to_host()) for n in replayed)
 
 
+def test_scoring_capture_keeps_its_buffers():
+    """What a captured run let go of (its quantised hidden states) is not given
+    to tensors made later: a replay leaves them as they are."""
+    stream = torch.cuda.Stream()
+    ctx = Context(0, stream=stream.cuda_stream)
+    tokens, hidden, vocab = 6, 384, 4001
+    h, w = randn(tokens, hidden, seed=1), randn(vocab, hidden, seed=2) * 0.05
+    target = torch.randint(0, vocab, (tokens,), generator=gen(3), device="cuda")
+    torch.cuda.synchronize()
+    head = scoring.quantize_fp8(dev(ctx, w), block_rows=128)
+    score(ctx, h, head, target, 3)
+    ctx.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got, logits = score(ctx, h, head, target, 3)
+    others = [randn(tokens, hidden, seed=s) for s in (7, 8, 9)]
+    torch.cuda.synchronize()
+    later = [scoring.quantize_fp8(dev(ctx, x)) for x in others]
+    before = [m.q.to_host() for m in later]
+    h.copy_(randn(tokens, hidden, seed=5))
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(np.array_equal(b, m.q.to_host()) for b, m in zip(before, later))
+
+
 @pytest.mark.parametrize("tokens, other", [(40, 40), (1, 1500), (1500, 200)])
 def test_scoring_on_two_streams(tctx, tokens, other):
     """Two contexts on one GPU, working at the same time on their own streams,
