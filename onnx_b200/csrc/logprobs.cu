@@ -207,11 +207,31 @@ struct Row {
     }
 };
 
-// A descending list with the keys of the lanes in `todo`.  (Not inlined: it is
-// called where few warps go, and its code would be many times the scan's.)
-__device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned todo, int lane) {
+// The k best of a descending list and the keys of the lanes in `todo`, descending
+// (and perhaps more after them).  (Not inlined: it is called where few warps go,
+// and its code would be many times the scan's.)
+__device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned todo, int k, int lane) {
+    const int n = __popc(todo);
+    if (n > k && k <= 12) {
+        // k times the best of all: a k-th of the work of an insertion for each key
+        if (!(todo >> lane & 1)) key = 0;
+        uint64_t mine = 0;
+        for (int i = 0; i < k; ++i) {
+            const bool from_list = list > key;
+            const uint64_t cand = from_list ? list : key;
+            const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(cand >> 32));
+            const uint32_t lo = __reduce_max_sync(kAll, (uint32_t)(cand >> 32) == hi ? (uint32_t)cand : 0u);
+            const uint64_t won = (uint64_t)hi << 32 | lo;
+            if (cand == won) {  // (keys differ; 0, no entry, may stay)
+                if (from_list) list = 0;
+                else key = 0;
+            }
+            if (lane == i) mine = won;
+        }
+        return mine;
+    }
     // sorting and merging cost about as much as 6 single insertions
-    if (__popc(todo) > 6) {
+    if (n > 6) {
         key = sort_desc(todo >> lane & 1 ? key : 0, lane);
         return __any_sync(kAll, list != 0) ? merge_desc(list, key, lane) : key;
     }
@@ -246,7 +266,7 @@ struct Warp {
     }
     // keys of lanes in `todo` into the list
     __device__ __forceinline__ void insert(uint64_t key, unsigned todo, int lane) {
-        list = with_keys(list, key, todo, lane);
+        list = with_keys(list, key, todo, k, lane);
         kth = __shfl_sync(kAll, list, k - 1);
         const uint32_t o = (uint32_t)(kth >> 32);
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
@@ -270,14 +290,16 @@ struct Warp {
         w2 = fma2(e, pack2(fmaxf(u.x, -FLT_MAX), fmaxf(u.y, -FLT_MAX)), w2);
     }
     template <typename T>
-    __device__ __forceinline__ void sum(const Row<T> &, const uint4 (&raw)[U]) {
+    __device__ __forceinline__ void sum(const Row<T> &, const uint4 (&raw)[U], uint32_t left) {  // of the row, for the warp
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            if (32 * u >= left) break;
 #pragma unroll
             for (int i = 0; i < Row<T>::VN / 2; ++i) {
                 const float2 p = Row<T>::pair(raw[u], i);
                 add(p.x, p.y);
             }
+        }
     }
     // A group: `best` its largest element, first its first index, exact() its best
     // element's key, `here` whether the lane has one.  It can enter the list if it
@@ -330,24 +352,34 @@ struct Args {
 };
 
 // The list of groups to one of elements: lanes with `group` hold theirs in `raw`
-// (vectors at + 32 u), others the key of a group of one element or 0 in `single`.
+// (vectors at + 32 u, no warp's beyond 32 u >= left), others the key of a group of
+// one element or 0 in `single`.
 template <typename T>
 __device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, const uint4 (&raw)[U], uint32_t at,
-                                              bool group, uint64_t single, int lane) {
+                                              bool group, uint64_t single, int lane, uint32_t left = 32 * U) {
     const uint64_t mine = group ? r.best_key(raw, Row<T>::best(raw), at) : single;
     st.list = 0;
     st.insert(mine, kAll, lane);  // the best of each group first
+    // then what else reaches the k-th, an element a lane at a time, read again by
+    // its index (the loop's body once per element in the code took longer than
+    // the rows' memory: instruction cache)
+    uint32_t todo = 0;
 #pragma unroll
     for (int j = 0; j < Row<T>::N; j += 2) {
+        if (32 * (j / Row<T>::VN) >= left) break;
         const float2 p = Row<T>::pair(raw[j / Row<T>::VN], j % Row<T>::VN / 2);
-        if (!__any_sync(kAll, group && !(p.x < st.thr && p.y < st.thr))) continue;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint64_t key = make_key(e ? p.y : p.x, r.index(at, j + e));
-            const bool want = group && at + 32 * (j / Row<T>::VN) < r.nvec && key > st.kth && key != mine;
-            const unsigned todo = __ballot_sync(kAll, want);
-            if (todo) st.insert(key, todo, lane);
-        }
+        todo |= (!(p.x < st.thr) ? 1u : 0u) << j | (!(p.y < st.thr) ? 1u : 0u) << (j + 1);
+    }
+    if (!group) todo = 0;
+    while (__any_sync(kAll, todo != 0)) {
+        const int j = todo ? __ffs(todo) - 1 : 0;
+        const uint32_t idx = r.index(at, j);
+        bool want = todo && at + 32 * (j / Row<T>::VN) < r.nvec;
+        todo &= todo - 1;
+        const uint64_t key = want ? make_key(to_f32(r.x[idx]), idx) : 0;
+        want = want && key > st.kth && key != mine;
+        const unsigned lanes = __ballot_sync(kAll, want);
+        if (lanes) st.insert(key, lanes, lane);
     }
 }
 template <typename T>
@@ -431,7 +463,7 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
     uint4 next[U];
     if (v0 < r.nvec) r.load(next, v0 + lane);
     while (v0 < r.nvec) {
-        const uint32_t at = v0 + lane;
+        const uint32_t at = v0 + lane, left = r.nvec - v0;
         uint4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = next[u];
@@ -445,7 +477,7 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
         const float best = Row<T>::best(raw);
         const bool changed = st.offer(best, at < r.nvec, floor, lane, r.index(at, 0), [&] { return r.best_key(raw, best, at); });
         if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
-        st.sum(r, raw);
+        st.sum(r, raw, left);
     }
     if (w == nw - 1) edges(st, r, lane);
 }
@@ -470,8 +502,8 @@ __global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ 
                 r.load(raw, lane);
                 const float best = Row<T>::best(raw);
                 if (__any_sync(kAll, best > st.m)) st.raise(best);
-                list_elements(st, r, raw, lane, lane < r.nvec, 0, lane);
-                st.sum(r, raw);
+                list_elements(st, r, raw, lane, lane < r.nvec, 0, lane, r.nvec);
+                st.sum(r, raw, r.nvec);
                 edges(st, r, lane);
             }
         } else {
