@@ -21,15 +21,17 @@
 // best element's unless two groups of a chunk enter with the same value: chunks
 // are runs of the row, so between chunks either index gives the same order.  (A
 // list of elements took a comparison each and four times the insertions: one row
-// of 250037 floats with 20 alternatives took 33 us instead of 18, and 12 since
+// of 250037 floats with 20 alternatives took 33 us instead of 18, and 11 since
 // the warps share what they have reached and join in halves.)
 //
 // Bound by HBM (each logit is read once, 16 bytes a thread and load, the next
 // 64 bytes in flight while the last are summed).  Pairs of elements share their
 // additions, multiplications and FMAs (f32x2); per element that leaves about
 // 5 instructions and one base-2 exponential.  2048 x 250037 floats: 299 us
-// (6.8 TB/s), with 20 alternatives 324; bfloat16 161 us (6.3 TB/s), with 20
-// alternatives 216, where instructions for the lists bound it.
+// (6.8 TB/s), with 20 alternatives 319; bfloat16 164 us (6.2 TB/s), with 20
+// alternatives 223, where instructions for the lists bound it; short rows are
+// bound by a row's chain of loads and reductions (16384 x 1001 halves: 12 us,
+// with 20 alternatives 34).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -627,8 +629,8 @@ int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
     const T *x = static_cast<const T *>(xv);
     const int64_t row_bytes = (int64_t)g.vocab * (int)sizeof(T);
     // A warp to a row for short rows, or for enough of them to fill the SMs with
-    // warps (5000 x 20000 bfloat16, 5 alternatives: 73 us, 4 warps to a row 95, 8
-    // warps 127); 4 warps, as joining their lists leaves fewer idle, while SMs get
+    // warps (5000 x 20000 bfloat16, 5 alternatives: 65 us; before later steps 73, 4
+    // warps to a row 95, 8 warps 127); 4 warps, as joining their lists leaves fewer idle, while SMs get
     // 4 rows each (1000 x 10000: 19 us, 8 warps 25; 300 x 50000: 24 us, 8 warps 23).
     if (row_bytes <= 8192 || g.rows >= 24 * ctx->num_sms) {
         const unsigned grid = (unsigned)std::min<int64_t>((g.rows + 7) / 8, 1 << 30);
