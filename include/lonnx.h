@@ -166,8 +166,8 @@ LONNX_API int lonnx_conv2d_f32(lonnx_ctx *ctx, const float *x, const float *w, c
  * pointer, where lonnx_gemm_fp8 is to read it); scale: [rows or ceil(rows /
  * 128), ceil(cols / 128)] at leading dimension lds.  Bytes of q and scale past
  * a row's end are left as they are.  NaN stays NaN and does not touch its
- * block's scale; an infinity makes its whole block NaN (scale infinite).  No
- * counterpart in the reference. */
+ * block's scale; an infinity makes its whole block NaN (scale infinite).  x, q
+ * and scale do not overlap.  No counterpart in the reference. */
 LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
                                  int block_rows, void *q, int64_t ldq, float *scale, int64_t lds);
 /* C = act(A . B^T + bias) with 8-bit float operands (e4m3) and block scales:
@@ -182,7 +182,7 @@ LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64
  * is summed by the tensor cores, blocks are scaled and summed in fp32, and the
  * result is rounded to C's type once, after the epilogue (lonnx_gemm_f32's,
  * whose ReLU gives 0 for NaN).  K = 0 gives the bias through the activation.
- * Sizes up to 2^30.  The order of the sums is fixed by the sizes: the same
+ * Sizes up to 2^30.  C overlaps none of the inputs.  The order of the sums is fixed by the sizes: the same
  * call gives the same bits.  Runs without workspace.  lonnx_gemm_f32's
  * counterpart for quantised weights. */
 LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t lda, const float *scaleA, int64_t ldsA,
@@ -207,8 +207,9 @@ LONNX_API int lonnx_softmax_f32(lonnx_ctx *ctx, const float *x, float *y, int64_
  * -inf have no probability; where a row has nothing else, its logprob and
  * top_logprob are -inf and its entropy 0.  A NaN or +inf logit makes the row's
  * log-probabilities and entropy NaN; among the alternatives NaN comes last.
- * temperature: 0.001 to 1000.  The row kernel next to lonnx_softmax_f32 for
- * vocabularies; no counterpart in the reference. */
+ * temperature: 0.001 to 1000.  No output overlaps another or an input.  The
+ * row kernel next to lonnx_softmax_f32 for vocabularies; no counterpart in the
+ * reference. */
 LONNX_API int lonnx_token_logprobs(lonnx_ctx *ctx, const void *logits, int dtype, int64_t rows, int64_t vocab,
                                    int64_t ld, const int64_t *targets, float temperature, float *logprob,
                                    float *entropy, int k, float *top_logprob, int64_t *top_id);

@@ -12,7 +12,8 @@ and the likeliest alternatives:
 
 All take and give ``DeviceTensor``s and only enqueue work on the context's
 stream (``lonnx_quantize_fp8``, ``lonnx_gemm_fp8``, ``lonnx_token_logprobs``
-of include/lonnx.h, which has the formulas).
+of include/lonnx.h, which has the formulas).  A tensor to write (``out``)
+overlaps no other tensor of its call.
 """
 from __future__ import annotations
 
