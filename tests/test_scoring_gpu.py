@@ -442,6 +442,41 @@ def test_logprobs_offsets_past_32_bits(tctx):
     check_scores({n: t[-3:] for n, t in got.items()}, want, z, vocab, 1.0)
 
 
+@pytest.mark.parametrize("m, n, k", [(9000, 250048, 40), (9000, 250037, 40)])  # rows on 16 bytes, and not
+def test_product_offsets_past_32_bits(tctx, m, n, k):
+    """Rows that start more than 2^31 elements into C."""
+    a, sa, b, sb = fp8_operands(m, n, k, seed=n)
+    got = run_product(tctx, a, sa, b, sb, k, "bf16")
+    at = torch.tensor([0, 1, m // 2, m - 2, m - 1], device="cuda")
+    want, mag = product_reference(a[at], sa[at], b, sb, k)
+    assert ((got[at].double() - want).abs() <= product_bound(mag, k, "bf16", want)).all()
+
+
+def test_product_of_few_rows_offsets_past_32_bits(tctx):
+    m, n, k, ldc = 20, 1000, 384, (1 << 27) + 8
+    a, sa, b, sb = fp8_operands(m, n, k, seed=4)
+    got = run_product(tctx, a, sa, b, sb, k, "bf16", ldc=ldc).double()
+    want, mag = product_reference(a, sa, b, sb, k)
+    assert ((got - want).abs() <= product_bound(mag, k, "bf16", want)).all()
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_offsets_past_32_bits(tctx, block_rows, offset):
+    """Rows that start more than 2^31 elements into x and q."""
+    rows, cols, ld = 20, 300, (1 << 27) + 16
+    x = torch.empty(rows * ld + offset, dtype=torch.float16, device="cuda")
+    q = torch.empty(rows * ld + offset, dtype=torch.uint8, device="cuda")
+    part = torch.as_strided(x, (rows, cols), (ld, 1), offset)
+    part.copy_(randn(rows, cols, seed=5))
+    scale = torch.empty(-(-rows // block_rows), 3, device="cuda")
+    N.check(N.lib.lonnx_quantize_fp8(tctx.handle, x.data_ptr() + 2 * offset, 10, rows, cols, ld, block_rows,
+                                     q.data_ptr() + offset, ld, scale.data_ptr(), 3))
+    want, want_scale = quantize_reference(part, block_rows)
+    got = torch.as_strided(q, (rows, cols), (ld, 1), offset).contiguous().view(torch.float8_e4m3fn)
+    assert torch.equal(scale, want_scale) and torch.equal(got.double(), want)
+
+
 # ---- together -------------------------------------------------------------------
 
 def score(ctx, hidden, head, target, k, out=None):
