@@ -103,17 +103,23 @@ __device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, F
 // warp to a block, 4 elements a lane, was bound by instructions: 72 us instead
 // of 43 at 32768 x 1536 floats).  The next 64 bytes a thread are in flight
 // meanwhile.
+template <typename T>
+struct RowWalk {
+    static constexpr int VN = 16 / (int)sizeof(T);
+    static constexpr int LANES = 8, NV = QB / LANES / VN;
+    static constexpr int U = 4 / NV;            // blocks of a group of lanes at a time: 64 bytes a thread
+    static constexpr int GROUPS = 256 / LANES;  // of a CTA
+};
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, I rows, I cols,
                                                        uint8_t *__restrict__ q, int64_t ldq,
                                                        float *__restrict__ scale, int64_t lds) {
-    constexpr int VN = 16 / (int)sizeof(T);
-    constexpr int LANES = 8, NV = QB / LANES / VN;
-    constexpr int U = 4 / NV;  // blocks of a group of lanes at a time: 64 bytes a thread
+    using W = RowWalk<T>;
+    constexpr int VN = W::VN, LANES = W::LANES, NV = W::NV, U = W::U;
     const int lane = threadIdx.x % LANES;
     const I nkb = (cols + QB - 1) / QB;
-    const I groups = (I)gridDim.x * (256 / LANES), srow = groups / nkb, skb = groups - srow * nkb;
-    I b0 = (I)blockIdx.x * (256 / LANES) + (I)(threadIdx.x / LANES), row = b0 / nkb, kb = b0 - row * nkb;
+    const I groups = (I)gridDim.x * W::GROUPS, srow = groups / nkb, skb = groups - srow * nkb;
+    I b0 = (I)blockIdx.x * W::GROUPS + (I)(threadIdx.x / LANES), row = b0 / nkb, kb = b0 - row * nkb;
     const auto advance = [&] {  // to the block `groups` further on
         row += srow;
         kb += skb;
@@ -361,8 +367,13 @@ int quantize(lonnx_ctx *ctx, const void *xv, int64_t rows, int64_t cols, int64_t
             // the CTAs that an SM holds at once (by registers), each walking over blocks
             const int64_t total = rows * nkb;
             const unsigned grid = (unsigned)std::min<int64_t>((total + 31) / 32, ctx->num_sms * (sizeof(T) == 4 ? 4 : 3));
-            // 32-bit indices where blocks and columns allow it
-            if (total + grid * 64ll < (1ll << 31) && cols < (1ll << 30))
+            // 32-bit indices where blocks and columns allow it.  A group of lanes whose
+            // neighbour in the warp has the last block (3 blocks before its own) has U
+            // blocks at hand and U in flight, each a grid's groups further on, and has
+            // stepped past them: the furthest block whose row it computes.
+            using W = RowWalk<T>;
+            const int64_t furthest = total + 3 + (int64_t)2 * W::U * W::GROUPS * grid;
+            if (furthest < (1ll << 31) && cols < (1ll << 30))
                 k_quantize_rows<T, int><<<grid, 256, 0, st>>>(x, ldx, (int)rows, (int)cols, q, ldq, scale, lds);
             else
                 k_quantize_rows<T, int64_t><<<grid, 256, 0, st>>>(x, ldx, rows, cols, q, ldq, scale, lds);
