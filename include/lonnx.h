@@ -58,11 +58,17 @@ typedef struct lonnx_ctx lonnx_ctx;
 LONNX_API int lonnx_ctx_create(int device, lonnx_ctx **out);
 /* The same on a stream that the caller owns (a cudaStream_t of `device`; NULL
  * is the default stream) and keeps until the context is destroyed: work of
- * the context is then ordered with the caller's own on that stream.  Calls
- * recorded into a CUDA graph of the caller's need their buffers for as long as
- * the graph is replayed: blocks freed during the recording are kept for it,
- * later ones are the caller's to keep (and one call outside the recording first
- * lets the allocator fetch its memory). */
+ * the context is then ordered with the caller's own on that stream.
+ *
+ * The stream may be recorded into a CUDA graph of the caller's, which is then
+ * replayed on it, or ordered with it, while the context lives.  Memory of the
+ * context's allocator that is handed out or freed during the recording is the
+ * graph's until the graph and the executables made from it are destroyed: freed
+ * then or later, it goes to no other call before that.  What recorded calls are
+ * given from before the recording (inputs, weights, outputs, an lonnx_graph) is
+ * the caller's to keep.  Memory that the allocator has to fetch from the device
+ * cannot be fetched during a recording (the call returns LONNX_E_OOM): make the
+ * same calls once before it. */
 LONNX_API int lonnx_ctx_create_on_stream(int device, void *stream, lonnx_ctx **out);
 LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx);
 LONNX_API int lonnx_ctx_device(const lonnx_ctx *ctx);

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <string>
@@ -17,17 +18,32 @@ namespace lonnx {
 // Device-side error flags, one int each, read and cleared by lonnx_sync().
 enum DevFlag { FLAG_OOB = 0, FLAG_TIMEOUT = 1, FLAG_TARGET = 2, FLAG_COUNT = 4 };
 
+// One recording of the context's stream into a CUDA graph of the caller's.  The
+// graph holds it as a user object, as do the executables made from it: `gone` is
+// set (on a thread of the driver's) when the last of them is destroyed.
+struct Capture {
+    std::atomic<bool> gone{false};
+    std::atomic<int> owners{1};  // the allocator and the user object
+    bool bound = false;          // the graph holds it; if not, its blocks stay for good
+};
+
+struct Block {
+    size_t size = 0;
+    bool given_back = false;          // by its owner, but kept for its captures
+    std::vector<Capture *> captures;  // recordings that may have put its address into their graphs
+};
+
 struct Allocator {
     // Caching allocator: freed blocks are kept per exact rounded size and
     // reused, so a graph that runs repeatedly reaches a steady state with no
     // cudaMalloc/cudaFree on the execute path.
     std::multimap<size_t, void *> free_blocks;
-    std::unordered_map<void *, size_t> live;
-    // Blocks freed while a caller records the stream into a CUDA graph: the graph
-    // has their addresses, so only the same capture may use them again.  They
-    // stay live until the context goes.
-    std::multimap<size_t, void *> captured_blocks;
-    unsigned long long capture_id = 0;
+    std::unordered_map<void *, Block> live;
+    // Blocks handed out or given back while a caller records the stream into a CUDA
+    // graph may be in that graph.  Once given back they wait here, where only the
+    // same recording finds them again, until the graph is gone.
+    std::multimap<size_t, void *> kept;
+    std::vector<std::pair<unsigned long long, Capture *>> captures;  // by the recording's id
     size_t bytes_reserved = 0;
     size_t limit = 0;  // 0 = none; LONNX_MEM_LIMIT (bytes) caps reservations
 };

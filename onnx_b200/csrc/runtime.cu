@@ -4,6 +4,8 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <algorithm>
+
 #include "lonnx_internal.cuh"
 
 namespace lonnx {
@@ -52,44 +54,116 @@ static size_t round_size(size_t b) {
     return (b + g - 1) / g * g;
 }
 
-// The id of the capture that records the context's stream into a caller's CUDA
-// graph; 0 when there is none.
-static unsigned long long caller_capture(lonnx_ctx *ctx) {
+static void disown(Capture *c) {
+    if (c->owners.fetch_sub(1) == 1) delete c;
+}
+
+// The user object's end: the graph and its executables are destroyed and idle.
+static void CUDART_CB capture_gone(void *of) {
+    Capture *c = static_cast<Capture *>(of);
+    c->gone.store(true);
+    disown(c);
+}
+
+// The recording of the context's stream into a caller's CUDA graph, if there is
+// one.  (lonnx_graph_capture's own recordings hold their blocks themselves.)
+static Capture *caller_capture(lonnx_ctx *ctx) {
+    if (ctx->capturing) return nullptr;
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
-    if (cudaStreamGetCaptureInfo(ctx->stream, &status, &id) != cudaSuccess) cudaGetLastError();
-    return status == cudaStreamCaptureStatusActive ? id : 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo(ctx->stream, &status, &id, &graph) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    if (status != cudaStreamCaptureStatusActive) return nullptr;
+    Allocator &A = ctx->alloc;
+    for (auto &known : A.captures)
+        if (known.first == id) return known.second;
+    Capture *c = new Capture();
+    A.captures.emplace_back(id, c);
+    cudaUserObject_t object = nullptr;
+    if (cudaUserObjectCreate(&object, c, capture_gone, 1, cudaUserObjectNoDestructorSync) == cudaSuccess) {
+        c->owners.fetch_add(1);
+        c->bound = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) == cudaSuccess;
+        if (!c->bound) cudaUserObjectRelease(object, 1);
+    }
+    if (!c->bound) cudaGetLastError();
+    return c;
+}
+
+static void use_in(Block &b, Capture *c) {
+    for (Capture *known : b.captures)
+        if (known == c) return;
+    b.captures.push_back(c);
+}
+
+// Blocks of graphs that are gone: those that their owners gave back are free.
+static void reclaim(Allocator &A) {
+    for (size_t i = 0; i < A.captures.size();) {
+        Capture *c = A.captures[i].second;
+        if (!c->bound || !c->gone.load()) {
+            ++i;
+            continue;
+        }
+        for (auto it = A.live.begin(); it != A.live.end();) {
+            std::vector<Capture *> &of = it->second.captures;
+            of.erase(std::remove(of.begin(), of.end(), c), of.end());
+            if (!it->second.given_back || !of.empty()) {
+                ++it;
+                continue;
+            }
+            const auto range = A.kept.equal_range(it->second.size);
+            for (auto k = range.first; k != range.second; ++k)
+                if (k->second == it->first) {
+                    A.kept.erase(k);
+                    break;
+                }
+            A.free_blocks.emplace(it->second.size, it->first);
+            it = A.live.erase(it);
+        }
+        A.captures.erase(A.captures.begin() + i);
+        disown(c);
+    }
 }
 
 int ctx_alloc(lonnx_ctx *ctx, size_t bytes, void **out) {
     Allocator &A = ctx->alloc;
     const size_t sz = round_size(bytes);
-    if (!A.captured_blocks.empty()) {
-        const unsigned long long id = caller_capture(ctx);
-        if (id && id == A.capture_id) {
-            auto of = A.captured_blocks.find(sz);
-            if (of != A.captured_blocks.end()) {
-                *out = of->second;
-                A.captured_blocks.erase(of);
+    reclaim(A);
+    Capture *cap = caller_capture(ctx);
+    if (cap) {
+        // what this recording let go of, and no other had (in the order of its stream)
+        const auto range = A.kept.equal_range(sz);
+        for (auto k = range.first; k != range.second; ++k) {
+            Block &b = A.live[k->second];
+            if (b.captures.size() == 1 && b.captures[0] == cap) {
+                b.given_back = false;
+                *out = k->second;
+                A.kept.erase(k);
                 return LONNX_OK;
             }
-        } else {
-            A.captured_blocks.clear();  // that capture is over: its blocks stay its graph's
         }
     }
+    const auto hand_out = [&](void *p) {
+        Block &b = A.live[p];
+        b.size = sz;
+        if (cap) b.captures.push_back(cap);
+        *out = p;
+        return LONNX_OK;
+    };
     auto it = A.free_blocks.find(sz);
     if (it != A.free_blocks.end()) {
-        *out = it->second;
+        void *p = it->second;
         A.free_blocks.erase(it);
-        A.live[*out] = sz;
-        return LONNX_OK;
+        return hand_out(p);
     }
     if (A.limit && A.bytes_reserved + sz > A.limit)
         return set_error(LONNX_E_OOM, "allocation of %zu bytes exceeds LONNX_MEM_LIMIT (%zu reserved)",
                          bytes, A.bytes_reserved);
     void *p = nullptr;
     cudaError_t e = cudaMalloc(&p, sz);
-    if (e != cudaSuccess) {
+    if (e != cudaSuccess && !cap) {  // (a stream that is recorded cannot be waited for)
         cudaGetLastError();
         // release cached blocks and retry once
         cudaStreamSynchronize(ctx->stream);
@@ -99,35 +173,42 @@ int ctx_alloc(lonnx_ctx *ctx, size_t bytes, void **out) {
         }
         A.free_blocks.clear();
         e = cudaMalloc(&p, sz);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return set_error(LONNX_E_OOM, "cudaMalloc(%zu) failed: %s", sz, cudaGetErrorString(e));
-        }
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(LONNX_E_OOM, "cudaMalloc(%zu) failed: %s", sz, cudaGetErrorString(e));
     }
     A.bytes_reserved += sz;
-    A.live[p] = sz;
-    *out = p;
-    return LONNX_OK;
+    return hand_out(p);
 }
 
 int ctx_free(lonnx_ctx *ctx, void *p) {
     if (!p) return LONNX_OK;
     Allocator &A = ctx->alloc;
     auto it = A.live.find(p);
-    if (it == A.live.end()) return set_error(LONNX_E_BADARG, "lonnx_free: pointer %p not allocated by this context", p);
+    if (it == A.live.end() || it->second.given_back)
+        return set_error(LONNX_E_BADARG, "lonnx_free: pointer %p not allocated by this context", p);
     if (ctx->capturing) {
         ctx->capture_hold.push_back(p);  // stays live until the captured graph is released
         return LONNX_OK;
     }
-    if (const unsigned long long id = caller_capture(ctx)) {
-        if (id != A.capture_id) A.captured_blocks.clear();  // an earlier capture's, its graph's for good
-        A.captured_blocks.emplace(it->second, p);
-        A.capture_id = id;
+    reclaim(A);
+    if (Capture *cap = caller_capture(ctx)) use_in(it->second, cap);
+    if (!it->second.captures.empty()) {
+        it->second.given_back = true;
+        A.kept.emplace(it->second.size, p);
         return LONNX_OK;
     }
-    A.free_blocks.emplace(it->second, p);
+    A.free_blocks.emplace(it->second.size, p);
     A.live.erase(it);
     return LONNX_OK;
+}
+
+// A context's scratch outlives the calls that use it: a recorded call's stays
+// its graph's when it is grown.
+static void scratch_used(lonnx_ctx *ctx, void *scratch) {
+    if (!scratch) return;
+    if (Capture *cap = caller_capture(ctx)) use_in(ctx->alloc.live[scratch], cap);
 }
 
 int ctx_scratch(lonnx_ctx *ctx, size_t bytes, void **out) {
@@ -143,6 +224,7 @@ int ctx_scratch(lonnx_ctx *ctx, size_t bytes, void **out) {
         if (rc) return rc;
         ctx->scratch_bytes = bytes;
     }
+    scratch_used(ctx, ctx->scratch);
     *out = ctx->scratch;
     return LONNX_OK;
 }
@@ -159,6 +241,7 @@ int ctx_scratch2(lonnx_ctx *ctx, size_t bytes, void **out) {
         if (rc) return rc;
         ctx->scratch2_bytes = bytes;
     }
+    scratch_used(ctx, ctx->scratch2);
     *out = ctx->scratch2;
     return LONNX_OK;
 }
@@ -230,6 +313,7 @@ LONNX_API int lonnx_ctx_destroy(lonnx_ctx *ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (auto &kv : ctx->alloc.free_blocks) cudaFree(kv.second);
     for (auto &kv : ctx->alloc.live) cudaFree(kv.first);
+    for (auto &known : ctx->alloc.captures) disown(known.second);
     cudaFree(ctx->dev_flags);
     if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
