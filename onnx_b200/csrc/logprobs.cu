@@ -9,9 +9,13 @@
 //
 // in one pass over the row: a running maximum m with S and W rescaled when it
 // grows, and a sorted list of the k best groups of elements per warp.  All sums
-// are fp32; a thread adds at most vocab / 256 terms, the rest is a tree.  x - m
-// is taken before any scaling, so logits of the type's lowest value stay
-// ordinary numbers; -inf adds exactly zero.
+// are fp32: 64 terms of a thread in turn, which then go into the thread's total
+// with what that addition rounded off kept beside it, and a tree over threads.  So
+// the error does not grow with the vocabulary, nor with the elements that a
+// thread gets (a warp's row of 250037 equal logits under one peak: S is off by up
+// to 4e-6; by 2e-4 where all 3900 terms are added to one fp32 number).  x - m is
+// taken before any scaling, so logits of the type's lowest value stay ordinary
+// numbers; -inf adds exactly zero.
 //
 // The alternatives.  A group is what one lane loads at once, 64 bytes of a row;
 // its key is its best element under (value, lowest index first).  The k best
@@ -252,7 +256,7 @@ __device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned
 template <bool TOP>
 struct Warp {
     float m;            // running maximum, the same in every lane
-    uint64_t s2, w2;    // the lane's sums, in two halves
+    uint64_t s2, w2;    // the lane's sums since the last fold, in two halves
     uint64_t list;      // lane's entry of the descending list of groups
     uint64_t kth;       // the k-th entry; 0 while there are fewer
     float thr;          // its value, NaN while there are fewer
@@ -262,6 +266,7 @@ struct Warp {
     __device__ __forceinline__ void reset(float c_, int k_) {
         m = -FLT_MAX;
         s2 = w2 = list = kth = 0;
+        before() = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         thr = __uint_as_float(0x7fc00000u);
         c = c_;
         k = k_;
@@ -273,14 +278,35 @@ struct Warp {
         const uint32_t o = (uint32_t)(kth >> 32);
         thr = o ? unordered(o) : __uint_as_float(0x7fc00000u);
     }
+    // the lane's sums before the last fold: s, w, and what their additions rounded
+    // off (in shared memory: they are touched every 64 terms, and registers are short)
+    static __device__ __forceinline__ float4 &before() {
+        __shared__ float4 all[256];
+        return all[threadIdx.x];
+    }
+    // a + x with its rounding added to l
+    static __device__ __forceinline__ void add_exact(float &a, float &l, float x) {
+        const float t = a + x, b = t - a;
+        l += (a - (t - b)) + (x - b);
+        a = t;
+    }
+    // all sums so far, the last ones added
+    __device__ __forceinline__ float4 folded() {
+        const float2 a = unpack2(s2), b = unpack2(w2);
+        float4 f = before();
+        add_exact(f.x, f.z, a.x + a.y);
+        add_exact(f.y, f.w, b.x + b.y);
+        s2 = w2 = 0;
+        return f;
+    }
+    __device__ __forceinline__ void fold() { before() = folded(); }
     __device__ __forceinline__ void raise(float best) {
         const float top = unordered(__reduce_max_sync(kAll, ordered(best)));
-        const float2 s = unpack2(s2), w = unpack2(w2);
-        Softmax a{m, s.x, w.x}, b{m, s.y, w.y};
+        const float4 f = folded();
+        Softmax a{m, f.x, f.y}, l{m, f.z, f.w};
         rescale(a, top, c);
-        rescale(b, top, c);
-        s2 = pack2(a.s, b.s);
-        w2 = pack2(a.w, b.w);
+        rescale(l, top, c);
+        before() = make_float4(a.s, a.w, l.s, l.w);
         m = top;
     }
     __device__ __forceinline__ void add(float x, float y) {
@@ -329,9 +355,9 @@ struct Warp {
         return false;
     }
     // the warp's sums, the same in every lane
-    __device__ __forceinline__ Softmax total() const {
-        const float2 s = unpack2(s2), w = unpack2(w2);
-        Softmax a{m, s.x + s.y, w.x + w.y};
+    __device__ __forceinline__ Softmax total() {
+        const float4 f = folded();
+        Softmax a{m, f.x + f.z, f.y + f.w};
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             a.s += __shfl_xor_sync(kAll, a.s, o);
@@ -461,6 +487,7 @@ __device__ __forceinline__ void edges(Warp<TOP> &st, const Row<T> &r, int lane) 
 template <int NW, typename T, bool TOP>
 __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, uint32_t *reached) {
     const uint32_t step = nw * 32 * U;
+    constexpr uint32_t FOLD = 64 / (U * Row<T>::VN / 2);  // chunks: 64 terms in each half
     uint32_t v0 = w * 32 * U;
     uint4 next[U];
     if (v0 < r.nvec) r.load(next, v0 + lane);
@@ -480,6 +507,7 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
         const bool changed = st.offer(best, at < r.nvec, floor, lane, r.index(at, 0), [&] { return r.best_key(raw, best, at); });
         if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
         st.sum(r, raw, left);
+        if (!(v0 & step * (FOLD - 1))) st.fold();  // (step is a power of two)
     }
     if (w == nw - 1) edges(st, r, lane);
 }
