@@ -38,7 +38,7 @@ enum lonnx_status {
     LONNX_E_OOM = -3,         /* device allocation failed or hit LONNX_MEM_LIMIT */
     LONNX_E_CUDA = -4,        /* CUDA runtime error                              */
     LONNX_E_TIMEOUT = -5,     /* a device-side bounded wait expired              */
-    LONNX_E_OOB = -6,         /* a Gather index outside [-dim, dim)              */
+    LONNX_E_OOB = -6,         /* a Gather index or a target out of range         */
     LONNX_E_UNSUPPORTED = -7  /* op/dtype/attribute not supported                */
 };
 
@@ -209,7 +209,8 @@ LONNX_API int lonnx_softmax_f32(lonnx_ctx *ctx, const float *x, float *y, int64_
  * one pass, without workspace.  targets (NULL: none) may be given without
  * logprob; a negative target marks a padding row, which is not read: logprob
  * 0, entropy 0, top_id -1, top_logprob -inf.  A target past the vocabulary
- * gives NaN and makes the next lonnx_sync() return LONNX_E_OOB.  Logits of
+ * gives a logprob of NaN and makes the next lonnx_sync() return LONNX_E_OOB,
+ * whether or not logprob is wanted.  Logits of
  * -inf have no probability; where a row has nothing else, its logprob and
  * top_logprob are -inf and its entropy 0.  A NaN or +inf logit makes the row's
  * log-probabilities and entropy NaN; among the alternatives NaN comes last.

@@ -429,14 +429,15 @@ __device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t r
     const bool none = a.s == 0.0f;  // every logit -inf: no token has any probability
     const float log_s = logf(a.s);
     if (lane == 0) {
-        if (g.targets && g.logprob) {
+        if (g.targets) {
             const int64_t t = g.targets[row];
-            float lp = __uint_as_float(0x7fc00000u);
-            if (t < (int64_t)g.vocab)
-                lp = none ? -INFINITY : fmaf(to_f32(r.x[t]) - a.m, g.inv_t, -log_s);
-            else
-                atomicExch(g.flags + lonnx::FLAG_TARGET, 1);
-            g.logprob[row] = lp;
+            const bool valid = t < (int64_t)g.vocab;
+            if (!valid) atomicExch(g.flags + lonnx::FLAG_TARGET, 1);
+            if (g.logprob) {
+                float lp = __uint_as_float(0x7fc00000u);
+                if (valid) lp = none ? -INFINITY : fmaf(to_f32(r.x[t]) - a.m, g.inv_t, -log_s);
+                g.logprob[row] = lp;
+            }
         }
         if (g.entropy) g.entropy[row] = none ? 0.0f : fmaf(a.w / a.s, -0.69314718055994530942f, log_s);
     }

@@ -3,6 +3,7 @@ SM on) and long, against 64 bits.  Most rows are padding, which is not read."""
 import pytest
 import torch
 
+from onnx_b200 import _native as N
 from onnx_b200.tensor import Context
 from test_scoring_gpu import TORCH, U, check_scores, gen, randn, run_scores, scores_reference
 
@@ -121,3 +122,27 @@ def test_many_rows_without_tokens_and_nan(tctx, vocab):
     assert got["top_id"][2, 0] == vocab // 2 and got["top_id"][3].tolist() == [0, 1, 2, 3]
     want, z = scores_reference(x[4:], target[4:], 4, 1.0)
     check_scores({n: t[4:] for n, t in got.items()}, want, z, vocab, 1.0)
+
+# ---- targets past the vocabulary ------------------------------------------------
+
+def entropies(ctx, x, target):
+    entropy = torch.empty(len(x), device="cuda")
+    N.check(N.lib.lonnx_token_logprobs(ctx.handle, x.data_ptr(), 1, len(x), x.shape[1], x.shape[1], target.data_ptr(),
+                                       1.0, None, entropy.data_ptr(), 0, None, None))
+    return entropy
+
+
+@pytest.mark.parametrize("rows, vocab", [(3, 700), (3, 12345), (3600, 2500)])
+def test_target_past_the_vocabulary_without_its_logprob(tctx, rows, vocab):
+    """Targets may be given for the padding alone; one past the vocabulary is reported all the same."""
+    x = randn(rows, vocab, seed=3)
+    target = torch.ones(rows, dtype=torch.int64, device="cuda")
+    target[1] = vocab
+    entropy = entropies(tctx, x, target)
+    with pytest.raises(N.LonnxError) as e:
+        tctx.sync()
+    assert e.value.code == -6 and "target" in e.value.message
+    assert entropy.isfinite().all()
+    target[1] = vocab - 1
+    entropies(tctx, x, target)
+    tctx.sync()
