@@ -381,10 +381,13 @@ LONNX_API int lonnx_sync(lonnx_ctx *ctx) {
     LONNX_CUDA(cudaMemcpy(flags, ctx->dev_flags, sizeof(flags), cudaMemcpyDeviceToHost));
     if (flags[FLAG_OOB] || flags[FLAG_TIMEOUT] || flags[FLAG_TARGET]) {
         LONNX_CUDA(cudaMemset(ctx->dev_flags, 0, sizeof(flags)));
+        char timeout[64] = "";
         if (flags[FLAG_TIMEOUT])
-            return set_error(LONNX_E_TIMEOUT, "a device-side pipeline wait expired (code %d)", flags[FLAG_TIMEOUT]);
-        if (flags[FLAG_OOB]) return set_error(LONNX_E_OOB, "Gather: an index was outside the bounds of the data axis");
-        return set_error(LONNX_E_OOB, "token_logprobs: a target was outside the vocabulary");
+            snprintf(timeout, sizeof(timeout), "a device-side pipeline wait expired (code %d)", flags[FLAG_TIMEOUT]);
+        const char *gather = flags[FLAG_OOB] ? "Gather: an index was outside the bounds of the data axis" : "";
+        const char *target = flags[FLAG_TARGET] ? "token_logprobs: a target was outside the vocabulary" : "";
+        return set_error(flags[FLAG_TIMEOUT] ? LONNX_E_TIMEOUT : LONNX_E_OOB, "%s%s%s%s%s", timeout,
+                         *timeout && (*gather || *target) ? "; " : "", gather, *gather && *target ? "; " : "", target);
     }
     return LONNX_OK;
 }

@@ -146,3 +146,26 @@ def test_target_past_the_vocabulary_without_its_logprob(tctx, rows, vocab):
     target[1] = vocab - 1
     entropies(tctx, x, target)
     tctx.sync()
+
+
+def test_sync_reports_every_flag(tctx):
+    """A Gather index and a target out of range before one sync: both are named."""
+    x = randn(3, 100)
+    entropies(tctx, x, torch.tensor([1, 100, 2], device="cuda"))
+    data, y = randn(4, 8), torch.empty(1, 8, device="cuda")
+    N.check(N.lib.lonnx_gather(tctx.handle, data.data_ptr(), 4, 1, 4, 8, torch.tensor([9], device="cuda").data_ptr(), 1,
+                               y.data_ptr()))
+    with pytest.raises(N.LonnxError) as e:
+        tctx.sync()
+    assert e.value.code == -6 and "Gather" in e.value.message and "target" in e.value.message
+    tctx.sync()
+
+
+def test_sync_reports_an_expired_wait_with_the_rest(tctx):
+    x = randn(3, 100)
+    entropies(tctx, x, torch.tensor([1, 100, 2], device="cuda"))
+    N.check(N.lib.lonnx_debug_expire_wait(tctx.handle, 100000))
+    with pytest.raises(N.LonnxError) as e:
+        tctx.sync()
+    assert e.value.code == -5 and "wait expired" in e.value.message and "target" in e.value.message
+    tctx.sync()
