@@ -26,6 +26,7 @@ from .tensor import BFLOAT16, FLOAT8E4M3, ONNX_DTYPE, Context, DeviceTensor
 
 BLOCK = 128          # columns of a quantisation block, and rows of a weight's
 MAX_ALTERNATIVES = 32
+MAX_SIZE = 1 << 30  # of a product, each way (32-bit arguments of the library)
 F32, I64 = (np.dtype(np.float32),), (np.dtype(np.int64),)
 FP8 = (FLOAT8E4M3,)
 FLOAT_TYPES = F32 + (np.dtype(np.float16), BFLOAT16)
@@ -108,6 +109,8 @@ def matmul_fp8(a: Fp8Matrix, w: Fp8Matrix, bias: DeviceTensor | None = None, act
     _need(a.q, "a", ctx, FP8)
     _need(w.q, "w", ctx, FP8)
     (m, lda), (n, ldw) = a.q.shape, w.q.shape
+    if max(m, n, k) > MAX_SIZE:
+        raise ValueError(f"{m} x {n} x {k}: at most 2^30 each")
     kb = -(-k // BLOCK)
     _need(a.scale, "a scale", ctx, F32, (m, kb))
     _need(w.scale, "w scale", ctx, F32, (-(-n // BLOCK), kb))
