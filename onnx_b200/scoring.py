@@ -94,10 +94,11 @@ def quantize_fp8(x: DeviceTensor, block_rows: int = 1, out=None) -> Fp8Matrix:
 
 
 def matmul_fp8(a: Fp8Matrix, w: Fp8Matrix, bias: DeviceTensor | None = None, activation: str | None = None,
-               dtype=np.float32, out: DeviceTensor | None = None) -> DeviceTensor:
+               dtype=None, out: DeviceTensor | None = None) -> DeviceTensor:
     """act(a . w^T + bias) [a.rows, w.rows] from activations ``a``
     (``block_rows=1``) and weights ``w`` (``block_rows=128``) over the same
-    columns; ``activation``: None, "relu" or "gelu"."""
+    columns; ``activation``: None, "relu" or "gelu"; ``dtype``: the result's,
+    float32 where neither it nor ``out`` says another."""
     ctx = a.q.ctx
     if a.block_rows != 1 or w.block_rows != BLOCK:
         raise ValueError(f"blocks of {a.block_rows} and {w.block_rows} rows: a needs 1, w {BLOCK}")
@@ -119,8 +120,10 @@ def matmul_fp8(a: Fp8Matrix, w: Fp8Matrix, bias: DeviceTensor | None = None, act
     if bias is not None:
         _need(bias, "bias", ctx, F32, (n,))
     if out is None:
-        out = DeviceTensor(ctx, (m, n), dtype)
+        out = DeviceTensor(ctx, (m, n), F32[0] if dtype is None else dtype)
     _need(out, "out", ctx, FLOAT_TYPES, (m, n))
+    if dtype is not None and np.dtype(dtype) != out.dtype:
+        raise ValueError(f"dtype: {np.dtype(dtype)} asked for, out has {out.dtype}")
     rc = _gemm(ctx.handle, a.q.ptr, lda, a.scale.ptr, kb, w.q.ptr, ldw, w.scale.ptr, kb,
                None if bias is None else bias.ptr, out.ptr, ONNX_DTYPE[out.dtype], n, m, n, k, ACTIVATIONS[activation])
     if rc:
