@@ -106,10 +106,6 @@ __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bul
 __device__ __forceinline__ void bulk_wait_group_read0() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
-// the same of all but the last committed group
-__device__ __forceinline__ void bulk_wait_group_read1() {
-    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-}
 // this thread's committed bulk stores are complete
 __device__ __forceinline__ void bulk_wait_group0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
