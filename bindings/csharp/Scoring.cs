@@ -14,9 +14,9 @@ public sealed class Fp8Matrix
     public DeviceBuffer Scale { get; init; } = null!;
     public int Rows { get; init; }
     public int Cols { get; init; }
-    public int Ld { get; init; }
+    public long Ld { get; init; }
     public int BlockRows { get; init; }
-    public int ScaleLd => (Cols + 127) / 128;
+    public long ScaleLd => ((long)Cols + 127) / 128;
 }
 
 public static class Scoring
@@ -26,11 +26,12 @@ public static class Scoring
     /// <summary>x [rows, cols] of element type dtype (Native.DT_*) in 8 bits; blockRows: 1 (activations) or 128 (weights).</summary>
     public static Fp8Matrix Quantize(CudaContext ctx, IntPtr x, int dtype, int rows, int cols, int blockRows = 1)
     {
-        int ld = (cols + 15) / 16 * 16, scales = (cols + Block - 1) / Block;
+        if (blockRows != 1 && blockRows != Block) throw new ArgumentException($"blockRows: 1 or {Block}, got {blockRows}");
+        long ld = ((long)cols + 15) / 16 * 16, scales = ((long)cols + Block - 1) / Block;
         var m = new Fp8Matrix
         {
             Q = new DeviceBuffer(ctx, (long)rows * ld),
-            Scale = new DeviceBuffer(ctx, (long)((rows + blockRows - 1) / blockRows) * scales * sizeof(float)),
+            Scale = new DeviceBuffer(ctx, ((long)rows + blockRows - 1) / blockRows * scales * sizeof(float)),
             Rows = rows, Cols = cols, Ld = ld, BlockRows = blockRows
         };
         Native.Check(Native.lonnx_quantize_fp8(ctx.Handle, x, dtype, rows, cols, cols, blockRows, m.Q.Ptr, ld,
