@@ -32,6 +32,15 @@ public sealed class CudaContext : SafeHandle
         Device = device;
     }
 
+    /// <summary>A context on a stream of the caller's (a cudaStream_t of `device`, IntPtr.Zero: the default one),
+    /// which is kept until the context is released.</summary>
+    public CudaContext(int device, IntPtr stream) : base(IntPtr.Zero, true)
+    {
+        Native.Check(Native.lonnx_ctx_create_on_stream(device, stream, out var h));
+        SetHandle(h);
+        Device = device;
+    }
+
     /// <summary>The process-wide context of one GPU (created on first use).</summary>
     public static CudaContext Default(int device = 0) => defaults.GetOrAdd(device, d => new CudaContext(d));
 

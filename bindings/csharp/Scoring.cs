@@ -39,24 +39,29 @@ public static class Scoring
         return m;
     }
 
-    /// <summary>act(a . w^T + bias) [a.Rows, w.Rows] into c (element type dtype); bias: floats or IntPtr.Zero.</summary>
-    public static void MatMul(CudaContext ctx, Fp8Matrix a, Fp8Matrix w, IntPtr bias, IntPtr c, int dtype, int epilogue = 0)
+    /// <summary>
+    /// act(a . w^T + bias) [a.Rows, w.Rows] into c (element type dtype, rows ldc elements apart, 0: w.Rows); bias:
+    /// floats or IntPtr.Zero.
+    /// </summary>
+    public static void MatMul(CudaContext ctx, Fp8Matrix a, Fp8Matrix w, IntPtr bias, IntPtr c, int dtype,
+        int epilogue = 0, long ldc = 0)
     {
         if (a.BlockRows != 1 || w.BlockRows != Block || a.Cols != w.Cols)
             throw new ArgumentException("a has blocks of 1 row, w of 128, over the same columns");
         Native.Check(Native.lonnx_gemm_fp8(ctx.Handle, a.Q.Ptr, a.Ld, a.Scale.Ptr, a.ScaleLd, w.Q.Ptr, w.Ld, w.Scale.Ptr,
-            w.ScaleLd, bias, c, dtype, w.Rows, a.Rows, w.Rows, a.Cols, epilogue));
+            w.ScaleLd, bias, c, dtype, ldc == 0 ? w.Rows : ldc, a.Rows, w.Rows, a.Cols, epilogue));
     }
 
     /// <summary>
     /// Log-probabilities of `targets` (int64 per row, negative: a padding row; IntPtr.Zero: none), entropies and
-    /// the k likeliest tokens of logits [rows, vocab]; an output that is IntPtr.Zero is not computed.
+    /// the k likeliest tokens of logits [rows, vocab], rows ld elements apart (0: vocab); an output that is
+    /// IntPtr.Zero is not computed.
     /// </summary>
     public static void TokenLogprobs(CudaContext ctx, IntPtr logits, int dtype, int rows, int vocab, IntPtr targets,
         IntPtr logprob, IntPtr entropy, int k = 0, IntPtr topLogprob = default, IntPtr topId = default,
-        float temperature = 1.0f)
+        float temperature = 1.0f, long ld = 0)
     {
-        Native.Check(Native.lonnx_token_logprobs(ctx.Handle, logits, dtype, rows, vocab, vocab, targets, temperature,
+        Native.Check(Native.lonnx_token_logprobs(ctx.Handle, logits, dtype, rows, vocab, ld == 0 ? vocab : ld, targets, temperature,
             logprob, entropy, k, topLogprob, topId));
     }
 }
