@@ -252,8 +252,10 @@ __device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned
     return list;
 }
 
-// What a warp has seen of its row.
-template <bool TOP>
+// What a warp has seen of its row.  LONG: a lane may get more than 64 terms in
+// each half, so its sums are folded (short rows do without: 16384 x 1001 halves
+// 11.6 us instead of 12.5).
+template <bool TOP, bool LONG>
 struct Warp {
     float m;            // running maximum, the same in every lane
     uint64_t s2, w2;    // the lane's sums since the last fold, in two halves
@@ -266,7 +268,7 @@ struct Warp {
     __device__ __forceinline__ void reset(float c_, int k_) {
         m = -FLT_MAX;
         s2 = w2 = list = kth = 0;
-        before() = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if constexpr (LONG) before() = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         thr = __uint_as_float(0x7fc00000u);
         c = c_;
         k = k_;
@@ -302,11 +304,20 @@ struct Warp {
     __device__ __forceinline__ void fold() { before() = folded(); }
     __device__ __forceinline__ void raise(float best) {
         const float top = unordered(__reduce_max_sync(kAll, ordered(best)));
-        const float4 f = folded();
-        Softmax a{m, f.x, f.y}, l{m, f.z, f.w};
-        rescale(a, top, c);
-        rescale(l, top, c);
-        before() = make_float4(a.s, a.w, l.s, l.w);
+        if constexpr (LONG) {
+            const float4 f = folded();
+            Softmax a{m, f.x, f.y}, l{m, f.z, f.w};
+            rescale(a, top, c);
+            rescale(l, top, c);
+            before() = make_float4(a.s, a.w, l.s, l.w);
+        } else {
+            const float2 s = unpack2(s2), w = unpack2(w2);
+            Softmax a{m, s.x, w.x}, b{m, s.y, w.y};
+            rescale(a, top, c);
+            rescale(b, top, c);
+            s2 = pack2(a.s, b.s);
+            w2 = pack2(a.w, b.w);
+        }
         m = top;
     }
     __device__ __forceinline__ void add(float x, float y) {
@@ -356,8 +367,16 @@ struct Warp {
     }
     // the warp's sums, the same in every lane
     __device__ __forceinline__ Softmax total() {
-        const float4 f = folded();
-        Softmax a{m, f.x + f.z, f.y + f.w};
+        Softmax a{m, 0.0f, 0.0f};
+        if constexpr (LONG) {
+            const float4 f = folded();
+            a.s = f.x + f.z;
+            a.w = f.y + f.w;
+        } else {
+            const float2 s = unpack2(s2), w = unpack2(w2);
+            a.s = s.x + s.y;
+            a.w = w.x + w.y;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             a.s += __shfl_xor_sync(kAll, a.s, o);
@@ -382,8 +401,8 @@ struct Args {
 // The list of groups to one of elements: lanes with `group` hold theirs in `raw`
 // (vectors at + 32 u, no warp's beyond 32 u >= left), others the key of a group of
 // one element or 0 in `single`.
-template <typename T>
-__device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, const uint4 (&raw)[U], uint32_t at,
+template <typename T, bool LONG>
+__device__ __forceinline__ void list_elements(Warp<true, LONG> &st, const Row<T> &r, const uint4 (&raw)[U], uint32_t at,
                                               bool group, uint64_t single, int lane, uint32_t left = 32 * U) {
     const uint64_t mine = group ? r.best_key(raw, Row<T>::best(raw), at) : single;
     st.list = 0;
@@ -410,8 +429,8 @@ __device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, c
         if (lanes) st.insert(key, lanes, lane);
     }
 }
-template <typename T>
-__device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, int lane) {
+template <typename T, bool LONG>
+__device__ __forceinline__ void list_elements(Warp<true, LONG> &st, const Row<T> &r, int lane) {
     // an element outside the vectors is a group of its own
     const uint32_t i = ~(uint32_t)st.list - r.head, vec = i / Row<T>::VN;
     const bool in = lane < st.k && st.list, group = in && ~(uint32_t)st.list >= r.head && vec < r.nvec;
@@ -423,9 +442,9 @@ __device__ __forceinline__ void list_elements(Warp<true> &st, const Row<T> &r, i
 
 // The row's answer from its sums and list of elements: one warp, every lane with
 // the same `a`.
-template <typename T, bool TOP>
-__device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t row, const Softmax &a, const Warp<TOP> &st,
-                                       int lane) {
+template <typename T, bool TOP, bool LONG>
+__device__ __forceinline__ void finish(const Args &g, const Row<T> &r, int64_t row, const Softmax &a,
+                                       const Warp<TOP, LONG> &st, int lane) {
     const bool none = a.s == 0.0f;  // every logit -inf: no token has any probability
     const float log_s = logf(a.s);
     if (lane == 0) {
@@ -466,8 +485,8 @@ __device__ __forceinline__ void finish_padding(const Args &g, int64_t row, int l
 }
 
 // the elements outside the vectors, one a lane
-template <typename T, bool TOP>
-__device__ __forceinline__ void edges(Warp<TOP> &st, const Row<T> &r, int lane) {
+template <typename T, bool TOP, bool LONG>
+__device__ __forceinline__ void edges(Warp<TOP, LONG> &st, const Row<T> &r, int lane) {
     if (r.head + r.tail == 0) return;
     const bool in = lane < r.head || (lane >= 16 && lane - 16 < r.tail);
     const uint32_t idx = lane < 16 ? lane : r.head + r.nvec * Row<T>::VN + lane - 16;
@@ -485,8 +504,8 @@ __device__ __forceinline__ void edges(Warp<TOP> &st, const Row<T> &r, int lane) 
 // ceil(k / NW)-th group so far.  Their least is reached by k groups of the row,
 // so groups below it cannot be in the answer: the warps' lists together then
 // take in about as many groups as one list over the whole CTA would.
-template <int NW, typename T, bool TOP>
-__device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int nw, int lane, uint32_t *reached) {
+template <int NW, typename T, bool TOP, bool LONG>
+__device__ __forceinline__ void scan(Warp<TOP, LONG> &st, const Row<T> &r, int w, int nw, int lane, uint32_t *reached) {
     const uint32_t step = nw * 32 * U;
     constexpr uint32_t FOLD = 64 / (U * Row<T>::VN / 2);  // chunks: 64 terms in each half
     uint32_t v0 = w * 32 * U;
@@ -508,13 +527,14 @@ __device__ __forceinline__ void scan(Warp<TOP> &st, const Row<T> &r, int w, int 
         const bool changed = st.offer(best, at < r.nvec, floor, lane, r.index(at, 0), [&] { return r.best_key(raw, best, at); });
         if (TOP && reached && changed && lane == (st.k + NW - 1) / NW - 1) *(volatile uint32_t *)(reached + w % NW) = (uint32_t)(st.list >> 32);
         st.sum(r, raw, left);
-        if (!(v0 & step * (FOLD - 1))) st.fold();  // (step is a power of two)
+        if (LONG && !(v0 & step * (FOLD - 1))) st.fold();  // (step is a power of two)
     }
     if (w == nw - 1) edges(st, r, lane);
 }
 
-// A warp per row
-template <typename T, bool TOP>
+// A warp per row (LONG: of more than kShortRow bytes)
+constexpr int kShortRow = 8192;
+template <typename T, bool TOP, bool LONG>
 __global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ x, Args g) {
     const int lane = threadIdx.x & 31;
     for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < g.rows; row += (int64_t)gridDim.x * 8) {
@@ -524,7 +544,7 @@ __global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ 
         }
         const Row<T> r(x + row * g.ld, g.vocab);
         const float c = g.inv_t * 1.44269504088896340736f;
-        Warp<TOP> st;
+        Warp<TOP, LONG> st;
         st.reset(c, g.k);
         if (TOP && r.nvec <= 32 * U) {
             // one chunk: its groups are here, so the list is of elements at once
@@ -538,10 +558,10 @@ __global__ void __launch_bounds__(256, 4) k_logprobs_warp(const T *__restrict__ 
                 edges(st, r, lane);
             }
         } else {
-            scan<1, T, TOP>(st, r, 0, 1, lane, nullptr);
+            scan<1>(st, r, 0, 1, lane, nullptr);
             if constexpr (TOP) list_elements(st, r, lane);
         }
-        finish<T, TOP>(g, r, row, st.total(), st, lane);
+        finish(g, r, row, st.total(), st, lane);
     }
 }
 
@@ -590,9 +610,9 @@ __global__ void __launch_bounds__(32 * NW, (TOP ? 32 : 24) / NW) k_logprobs_cta(
             if (threadIdx.x < NW) reached[threadIdx.x] = 0;
             __syncthreads();
         }
-        Warp<TOP> st;
+        Warp<TOP, true> st;
         st.reset(c, g.k);
-        scan<NW, T, TOP>(st, r, part * NW + w, parts * NW, lane, reached);
+        scan<NW>(st, r, part * NW + w, parts * NW, lane, reached);
         Softmax a = st.total();
         join_warps<NW, TOP>(joint, a, st.list, NW, w, lane, c);
         if (parts > 1) {
@@ -617,7 +637,7 @@ __global__ void __launch_bounds__(32 * NW, (TOP ? 32 : 24) / NW) k_logprobs_cta(
         }
         if (part == 0 && w == 0) {
             if constexpr (TOP) list_elements(st, r, lane);
-            finish<T, TOP>(g, r, row, a, st, lane);
+            finish(g, r, row, a, st, lane);
         }
         if (parts > 1) cluster.barrier_wait();
         __syncthreads();  // the next row's sums go into the same shared memory
@@ -661,9 +681,11 @@ int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
     // warps (5000 x 20000 bfloat16, 5 alternatives: 65 us; before later steps 73, 4
     // warps to a row 95, 8 warps 127); 4 warps, as joining their lists leaves fewer idle, while SMs get
     // 4 rows each (1000 x 10000: 19 us, 8 warps 25; 300 x 50000: 24 us, 8 warps 23).
-    if (row_bytes <= 8192 || g.rows >= 24 * ctx->num_sms) {
+    if (row_bytes <= kShortRow || g.rows >= 24 * ctx->num_sms) {
         const unsigned grid = (unsigned)std::min<int64_t>((g.rows + 7) / 8, 1 << 30);
-        k_logprobs_warp<T, TOP><<<grid, 256, 0, ctx->stream>>>(x, g);
+        // (a short row: at most 4 chunks, 64 terms, and one element outside the vectors)
+        const auto kernel = row_bytes <= kShortRow ? k_logprobs_warp<T, TOP, false> : k_logprobs_warp<T, TOP, true>;
+        kernel<<<grid, 256, 0, ctx->stream>>>(x, g);
         LONNX_CHECK_LAUNCH(ctx);
         return LONNX_OK;
     }
