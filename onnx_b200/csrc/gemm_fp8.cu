@@ -155,15 +155,18 @@ struct Wide {
 constexpr int kWideThreads = 640;
 constexpr int W_TMA = 16, W_MMA = 17, W_SCALE = 19;
 
-// Tiles in groups of `GROUP` rows of tiles, column by column within a group, so
+// Tiles in groups of `group` rows of tiles, column by column within a group, so
 // that the CTAs at work share both operands' tiles in L2.  Where C leaves by
-// element stores, its rows do not start on sectors, and a group is 4 rows: two
-// neighbours' halves of a sector meet in L2 (18651 x 17257 x 78 to bfloat16: 235
-// us, 299 in groups of 16; 1000 x 30001 x 2000 to halves: 105, 113 row by row).
-template <int GROUP>
-__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int &tm, int &tn) {
-    const int per = GROUP * tiles_n, g = t / per, first = g * GROUP;
-    const int h = min(GROUP, tiles_m - first), r = t - g * per;
+// element stores, its rows do not start on sectors, and neighbours' halves of a
+// sector have to meet in L2: groups of 1 row where K is one or two blocks and C's
+// bytes are all that counts (18651 x 17257 x 78 to floats: 341 us, 445 in groups
+// of 4; to bfloat16: 227, 247, 299 in groups of 16), of 4 rows for longer K, where
+// the operands' bytes count too (1000 x 30001 x 2000 to halves: 95 us, 99 row by
+// row; 300 x 50001 x 1024 to floats: 38.5, 42).
+__device__ __forceinline__ int tile_group(bool by_tma, int nkb) { return by_tma ? 16 : nkb <= 2 ? 1 : 4; }
+__device__ __forceinline__ void tile_at(int t, int group, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int per = group * tiles_n, g = t / per, first = g * group;
+    const int h = min(group, tiles_m - first), r = t - g * per;
     tn = r / h;
     tm = first + r - tn * h;
 }
@@ -175,7 +178,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                const float *__restrict__ sB, int64_t ldsB, const float *__restrict__ bias, T *__restrict__ C,
                int64_t ldc, int M, int N, int nkb, int epi, int *flags) {
     using W = Wide<BN>;
-    constexpr int GROUP = BY_TMA ? 16 : 4;
+    const int group = tile_group(BY_TMA, nkb);
     constexpr int S = W::S, SETS = W::SETS, COLS = 64;
     extern __shared__ __align__(1024) uint8_t base[];
     uint8_t *staging = base + S * W::STAGE;
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             if (lane == 0) {
                 for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                     int tm, tn;
-                    tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
+                    tile_at(t, group, tiles_m, tiles_n, tm, tn);
                     for (int b = 0; b < nkb; ++b, ++issued) {
                         const int s = issued % S;
                         if (!mbar_wait(empty(s), ((issued / S) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             for (int t = blockIdx.x, n = 0; t < tiles && ok; t += gridDim.x, ++n) {
                 const int set = SETS == 2 ? n & 1 : 0;
                 int tm, tn;
-                tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
+                tile_at(t, group, tiles_m, tiles_n, tm, tn);
                 const float *ra[4], *rb[NB];
                 float x[4], y[NB];
 #pragma unroll
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
             if (!ok) break;
             int tm, tn;
-            tile_at<GROUP>(t, tiles_m, tiles_n, tm, tn);
+            tile_at(t, group, tiles_m, tiles_n, tm, tn);
             const int row0 = tm * BM + q * 32, col0 = tn * BN + part * COLS;
             // bias and activation of columns [i, i + 32), in place
             auto finish = [&](int i) {
