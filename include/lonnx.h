@@ -8,8 +8,8 @@
  * maps a non-zero code to OpResult.Failure(op, lonnx_last_error())
  * (src/Lokad.Onnx.Backend/OpResult.cs:34-62) -- no entry point throws.
  *
- * Execution model: one lonnx_ctx per GPU = one device, one non-default CUDA
- * stream, one caching device allocator.  Op entry points only enqueue work on
+ * Execution model: one lonnx_ctx per GPU = one device, one CUDA stream (its
+ * own, or the caller's), one caching device allocator.  Op entry points only enqueue work on
  * the context's stream (device pointers in, device pointers out);
  * lonnx_sync() waits for it and reports errors the kernels flagged on the
  * device (out-of-range Gather index, bounded pipeline wait that expired).
@@ -188,9 +188,11 @@ LONNX_API int lonnx_quantize_fp8(lonnx_ctx *ctx, const void *x, int dtype, int64
  * is summed by the tensor cores, blocks are scaled and summed in fp32, and the
  * result is rounded to C's type once, after the epilogue (lonnx_gemm_f32's,
  * whose ReLU gives 0 for NaN).  K = 0 gives the bias through the activation.
- * Sizes up to 2^30.  C overlaps none of the inputs.  The order of the sums is fixed by the sizes: the same
- * call gives the same bits.  Runs without workspace.  lonnx_gemm_f32's
- * counterpart for quantised weights. */
+ * Sizes up to 2^30.  C overlaps none of the inputs.  The order of the sums is
+ * fixed by the sizes: the same call gives the same bits, but a row of A among
+ * more or fewer others may be summed in another order (and its GELU evaluated
+ * by another formula).  Runs without workspace.  lonnx_gemm_f32's counterpart
+ * for quantised weights. */
 LONNX_API int lonnx_gemm_fp8(lonnx_ctx *ctx, const void *A, int64_t lda, const float *scaleA, int64_t ldsA,
                              const void *B, int64_t ldb, const float *scaleB, int64_t ldsB, const float *bias,
                              void *C, int dtypeC, int64_t ldc, int M, int N, int K, int epilogue);

@@ -12,8 +12,8 @@
 // What bounds it.  8192^3: 0.52 ms in a burst (2130 TFLOP/s), 0.61 under the
 // power cap (1.47 GHz at 1 kW); a block of a 128 x 256 tile takes 860 cycles, of
 // which shared memory (operands written once and read once, 96 KB at 128 bytes a
-// cycle) needs 768 and the tensor cores 512.  32768 x 1536 x 384 to floats: 47 us,
-// 4.5 TB/s of output, with GELU 58, bound by the epilogue's instructions.
+// cycle) needs 768 and the tensor cores 512.  32768 x 1536 x 384 to floats: 46 us,
+// 4.4 TB/s of output, with GELU 59, bound by the epilogue's instructions.
 //
 // Two kernels.  k_fp8_wide: tiles of 128 rows of A x BN rows of B, for
 // problems that fill the GPU with them.  k_fp8_split: B's rows as the tensor

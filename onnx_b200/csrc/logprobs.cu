@@ -31,11 +31,12 @@
 // Bound by HBM (each logit is read once, 16 bytes a thread and load, the next
 // 64 bytes in flight while the last are summed).  Pairs of elements share their
 // additions, multiplications and FMAs (f32x2); per element that leaves about
-// 5 instructions and one base-2 exponential.  2048 x 250037 floats: 299 us
-// (6.8 TB/s), with 20 alternatives 319; bfloat16 164 us (6.2 TB/s), with 20
-// alternatives 223, where instructions for the lists bound it; short rows are
-// bound by a row's chain of loads and reductions (16384 x 1001 halves: 12 us,
-// with 20 alternatives 34).
+// 5 instructions and one base-2 exponential.  2048 x 250037 floats: 305 us
+// (6.7 TB/s), with 20 alternatives 330; bfloat16 172 us (6.0 TB/s), with 20
+// alternatives 222, where instructions for the lists bound it (4000 x 60000 floats
+// with 20: 178 us, 5.4 TB/s); short rows are bound by a row's chain of loads and
+// reductions (16384 x 1001 halves: 12.6 us, with 20 alternatives 34).  Folding the
+// sums costs long rows 1 to 4% of that.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -253,8 +254,8 @@ __device__ __noinline__ uint64_t with_keys(uint64_t list, uint64_t key, unsigned
 }
 
 // What a warp has seen of its row.  LONG: a lane may get more than 64 terms in
-// each half, so its sums are folded (short rows do without: 16384 x 1001 halves
-// 11.6 us instead of 12.5).
+// each half, so its sums are folded (short rows do without: 16384 x 1001 halves,
+// 2000 of them padding, 11.7 us instead of 12.5).
 template <bool TOP, bool LONG>
 struct Warp {
     float m;            // running maximum, the same in every lane
@@ -678,9 +679,10 @@ int launch(lonnx_ctx *ctx, const void *xv, const Args &g) {
     const T *x = static_cast<const T *>(xv);
     const int64_t row_bytes = (int64_t)g.vocab * (int)sizeof(T);
     // A warp to a row for short rows, or for enough of them to fill the SMs with
-    // warps (5000 x 20000 bfloat16, 5 alternatives: 65 us; before later steps 73, 4
-    // warps to a row 95, 8 warps 127); 4 warps, as joining their lists leaves fewer idle, while SMs get
-    // 4 rows each (1000 x 10000: 19 us, 8 warps 25; 300 x 50000: 24 us, 8 warps 23).
+    // warps (5000 x 20000 bfloat16, 5 alternatives: 67 us; when it was 73, 4 warps
+    // to a row took 95 and 8 warps 127); 4 warps, as joining their lists leaves
+    // fewer idle, while SMs get 4 rows each (1000 x 10000: 19 us, 8 warps 25; 300 x
+    // 50000: 24 us, 8 warps 23).
     if (row_bytes <= kShortRow || g.rows >= 24 * ctx->num_sms) {
         const unsigned grid = (unsigned)std::min<int64_t>((g.rows + 7) / 8, 1 << 30);
         // (a short row: at most 4 chunks, 64 terms, and one element outside the vectors)

@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, 
 // elements 4 lane .. 4 lane + 3 of each block to a lane (X4: as one load).  The
 // bytes leave as aligned words, put together from neighbouring lanes' and
 // blocks': L2 pays for each partly written 32-byte sector (single bytes, 8 to 32
-// in a row: 66 to 83 us at 11212 x 4229 halves).  Lane b takes the divisions of
+// in a row: 66 to 83 us at 11212 x 4229 halves; 53 us this way, and 47 at 11212 x
+// 4228 with one load for four elements).  Lane b takes the divisions of
 // block b.
 template <typename T, bool X4>
 __global__ void __launch_bounds__(256, 4) k_quantize_rows_any(const T *__restrict__ x, int64_t ldx, int64_t rows,
@@ -285,7 +286,9 @@ __global__ void __launch_bounds__(256, 4) k_quantize_rows_any(const T *__restric
 }
 
 // 128 x 128 blocks: a CTA of 16 warps per block, which stays in registers (32
-// values a thread) while the maximum crosses the CTA.
+// values a thread) while the maximum crosses the CTA.  250037 x 384 floats: 90 us,
+// 5.3 TB/s; bfloat16 84 us, 3.4 TB/s: a CTA has no load in flight from its
+// block's last one to its end, and only other CTAs' fill that time.
 constexpr int kBlockThreads = 512;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kBlockThreads, VEC && sizeof(T) == 2 ? 3 : 2)
