@@ -14,7 +14,8 @@
  * lonnx_sync() waits for it and reports errors the kernels flagged on the
  * device (out-of-range Gather index, bounded pipeline wait that expired).
  * A context is driven by one host thread at a time; contexts on different
- * GPUs are independent (batch sharding needs no collective).
+ * GPUs are independent (batch sharding needs no collective).  A call leaves the
+ * context's device as the calling thread's current one.
  *
  * Each op cites the reference routine it replaces (paths inside the
  * Lokad/Onnx project).

@@ -28,7 +28,9 @@ _DTYPES = {**{d: d for d in ONNX_DTYPE}, **{d.type: d for d in ONNX_DTYPE if d.t
 
 
 class Context:
-    """One GPU: device, CUDA stream and caching allocator (lonnx_ctx)."""
+    """One GPU: device, CUDA stream and caching allocator (lonnx_ctx).  Calls
+    leave its device as the thread's current one: a program with tensors of
+    another library on several devices names their device, or sets it again."""
 
     _default = {}
     _lock = threading.Lock()
