@@ -46,9 +46,17 @@ def test_32_bit_indices_hold_the_whole_walk():
     assert eval(rule, dict(total=2147455231, grid=444, u=2)) >= 2 ** 31
 
 
+@pytest.fixture
+def device_memory():
+    """Given back to the device afterwards, for tests in other processes."""
+    import torch
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [2147426000, 2147455231, 2147483647])
-def test_rows_up_to_the_last_32_bit_index(rows):
+def test_rows_up_to_the_last_32_bit_index(device_memory, rows):
     """One block a row in 16 bits; all but a few rows hold whatever the memory held."""
     import torch
 
